@@ -4,6 +4,8 @@ library; there is no CPU or PyTorch fallback."""
 from . import _lib  # noqa: F401  (fails loudly when the library is missing)
 from .cache import NativeRWKV7Cache, NativeRWKV7LegacyCache
 from .checkpoint import convert_state_dict, infer_config, load_checkpoint, to_upstream_state_dict, translate_name
+from .fp4 import (FP4Linear, dequantize_fp4, fp4_linear, fp4_scale_rows, fp4_scale_tiles, quantize_fp4,
+                  quantize_fp4_weight)
 from .gemm import dense_argmax, dense_linear
 from .install import install, uninstall
 from .lora import dense_small, fused_wa_lora, fused_wag_lora, fused_wavg_lora

@@ -79,6 +79,11 @@ SIGNATURES = {
     "rwkv7_tp_rows_resident": (I, [I, I]),
     "rwkv7_tp_attn_norm_mix6": (I, [P, P, P, P, P, P, PP, PP, PP, P, I, I, I, I, ctypes.c_longlong, I, F, I, I, P]),
     "rwkv7_tp_ffn_add_norm_mix": (I, [P] * 9 + [PP, P, I, I, I, I, ctypes.c_longlong, I, F, I, I, P]),
+    "rwkv7_fp4_scale_bytes": (L, [I, I, I]),
+    "rwkv7_fp4_quant": (I, [P, L, P, P, P, I, I, I, I, P]),
+    "rwkv7_fp4_dequant": (I, [P] * 4 + [I, I, I, I, P]),
+    "rwkv7_fp4_linear_workspace_bytes": (L, [I, I, I]),
+    "rwkv7_fp4_linear": (I, [P, L] + [P] * 7 + [L] + [I] * 6 + [P]),
     "rwkv7_a8w8_static_capacity_bytes": (L, []),
     "rwkv7_a8w8_linear_static": (I, [P] * 6 + [I, I, I, I, P]),
 }

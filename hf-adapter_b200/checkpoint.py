@@ -204,7 +204,7 @@ def to_upstream_state_dict(state_dict):
 def load_checkpoint(weights, *, dtype=torch.float16, device="cuda", quant=None, min_params: int = 8_000_000,
                     group_size: int = 128, state_dtype=torch.float32):
     """Build ``RWKV7ForCausalLM`` from upstream weights (a dict of tensors, or the path of a ``torch.save``d one),
-    cast to ``dtype``, optionally quantise the projections (``quant`` in {"mm4", "w8", "mm8", "a8w8"}) and move to
+    cast to ``dtype``, optionally quantise the projections (``quant`` in {"mm4", "w8", "mm8", "a8w8", "nvfp4", "mxfp4"}) and move to
     ``device``.  Returns the model in eval mode."""
     if not isinstance(weights, dict):
         weights = torch.load(weights, map_location="cpu", mmap=True, weights_only=True)

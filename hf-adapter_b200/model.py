@@ -332,8 +332,8 @@ class RWKV7ForCausalLM(nn.Module):
         """Final projection: logits ``[B,V]`` (all-gathered over the vocabulary shards when the head is sharded) or, with
         ``greedy``, the arg-max token of every row (local arg-max + one [B,2] exchange per rank)."""
         sharded = self.tp_shard_head and self.tp_group is not False
-        w = self.lm_head.weight
-        if greedy and _gemm.takes(xn, w) and int(xn.shape[0]) >= _gemm.MIN_ROWS:
+        w = getattr(self.lm_head, "weight", None)  # (None: a quantised head)
+        if greedy and w is not None and _gemm.takes(xn, w) and int(xn.shape[0]) >= _gemm.MIN_ROWS:
             # the arg-max rides in the head GEMM's epilogue: the logits are never written
             if not sharded:
                 return _gemm.dense_argmax(xn, w)

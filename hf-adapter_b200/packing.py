@@ -21,6 +21,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
+from . import fp4 as _fp4
 from . import gemm as _gemm
 from . import lora as _lora
 from . import norm_mix as _nm
@@ -30,7 +31,7 @@ from . import rows as _rowsk
 from ._util import zero_lists
 
 PACK_SLOTS = 41
-_QUANT_TYPES = (_q.MM4Linear, _q.MM8Linear, _q.A8W8Linear)
+_QUANT_TYPES = (_q.MM4Linear, _q.MM8Linear, _q.A8W8Linear, _fp4.FP4Linear)
 
 
 def graph_linear_operand(mod):

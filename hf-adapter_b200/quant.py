@@ -20,6 +20,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from . import fp4 as _fp4
 from . import rows as _rowsk
 from ._util import dt_code, ptr, require_cuda, stream_ptr
 
@@ -707,7 +708,8 @@ class A8W8Linear(torch.nn.Module):
 def quantize_model(model, kind: str, *, min_params: int = 8_000_000, group_size: int = 128, skip=("lm_head",)) -> int:
     """Swap eligible ``nn.Linear`` modules in place (role of quantize_model_mm8 / quantize_model_mm4,
     rwkv7_hf/native_quant_mm8.py:631-684, rwkv7_hf/native_quant_mm4.py:761-832).  ``kind`` in
-    {"mm8" (fp16i8 affine), "w8" (row-wise int8), "mm4" (int4 group-wise), "a8w8"}; modules with fewer than ``min_params`` weights or whose name is in ``skip`` stay dense."""
+    {"mm8" (fp16i8 affine), "w8" (row-wise int8), "mm4" (int4 group-wise), "a8w8", "nvfp4" / "mxfp4" (4-bit floating point for both
+    operands)}; modules with fewer than ``min_params`` weights or whose name is in ``skip`` stay dense."""
     n = 0
     for parent_name, parent in list(model.named_modules()):
         for name, child in list(parent.named_children()):
@@ -728,6 +730,10 @@ def quantize_model(model, kind: str, *, min_params: int = 8_000_000, group_size:
                 if child.in_features % 16 or child.out_features % 8:
                     continue
                 new = A8W8Linear(child)
+            elif kind in _fp4.FORMATS:
+                if child.in_features % 32:
+                    continue
+                new = _fp4.FP4Linear(child, format=kind)
             else:
                 raise ValueError(f"unknown quantisation kind {kind!r}")
             setattr(parent, name, new)

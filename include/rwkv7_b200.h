@@ -464,6 +464,30 @@ int rwkv7_tp_ffn_add_norm_mix(const void* residual, const void* partial, void* p
                               void* const* inbox_ptrs, void* counters, int rank, int world, int rows, int D,
                               long long slot_elems, int max_ctas, float eps, int wait_ms, int dtype, void* stream);
 
+/* ---- microscaled 4-bit floating point (no counterpart in the reference) ----
+ * Elements are E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign; nearest, ties to the even code), two a byte, the even element in
+ * the low nibble: packed [rows, K/2].  RWKV7_FP4_MX: 32 elements share 2^(byte - 127), byte = max(biased exponent of the
+ * block's largest magnitude - 2, 0).  RWKV7_FP4_NV: 16 elements share an E4M3 scale of (largest magnitude / g / 6), the row
+ * an fp32 factor g = 2^(floor(log2 of the row's largest magnitude) - 10) (any fp32 factor in a weight made elsewhere).
+ * A block with an element that is not finite gets a NaN scale (255 / 0x7f).
+ * Scales lie in tiles of 128 rows x 4 blocks, 512 bytes each: byte (row % 32) * 16 + row % 128 / 32 * 4 + block % 4 of tile
+ * [row / 128][block / 4] (rwkv7_fp4_scale_bytes bytes in all; what pads a tile is zero).
+ * x has rows ldx elements apart, each 16-byte aligned; K is a multiple of 32. */
+#define RWKV7_FP4_MX 0
+#define RWKV7_FP4_NV 1
+int64_t rwkv7_fp4_scale_bytes(int rows, int K, int format);
+int rwkv7_fp4_quant(const void* x, int64_t ldx, void* packed, void* scales, float* row_scale, int rows, int K, int format, int dtype,
+                    void* stream);
+int rwkv7_fp4_dequant(const void* packed, const void* scales, const float* row_scale, void* out, int rows, int K, int format, int dtype,
+                      void* stream);
+/* y [M,N] = epilogue(x_q [M,K] . w_q [N,K]^T (+ bias)): x is quantised on the way (rwkv7_fp4_quant into the workspace), both
+ * operands stay in 4 bits on the tensor cores, sums are fp32 and rounded once after the epilogue (relu(.)^2, or + residual).
+ * w_row_scale NULL = 1. */
+int64_t rwkv7_fp4_linear_workspace_bytes(int M, int K, int format);
+int rwkv7_fp4_linear(const void* x, int64_t ldx, const void* w_packed, const void* w_scales, const float* w_row_scale,
+                     const void* bias, const void* residual, void* y, void* workspace, int64_t workspace_bytes, int M, int K, int N,
+                     int epilogue, int format, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
