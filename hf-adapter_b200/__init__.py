@@ -27,6 +27,7 @@ from .recurrent import (dplr_chunk_scan, fused_recurrent_output_prepare, fused_r
                         fused_recurrent_scan_state_prep, fused_recurrent_update, native_fp16_recurrent_output_prepare_raw,
                         native_fp16_recurrent_should_use, native_fp16_sequence, self_chunk_rwkv7)
 
+from .sampling import process_logits, sample_tokens
 from .sharding import shard_spec, shard_state_dict
 from .tokenizer import RWKVWorldTokenizer
 from .state_pool import PoolDecodeGraph, PrefixEntry, RWKV7StatePool, StaleSlotError

@@ -84,6 +84,8 @@ SIGNATURES = {
     "rwkv7_fp4_dequant": (I, [P] * 4 + [I, I, I, I, P]),
     "rwkv7_fp4_linear_workspace_bytes": (L, [I, I, I]),
     "rwkv7_fp4_linear": (I, [P, L] + [P] * 7 + [L] + [I] * 6 + [P]),
+    "rwkv7_process_logits": (I, [P, L, P, P, L, I, I, I, P]),
+    "rwkv7_sample_tokens": (I, [P, L, P, P, P, L, P, P, I, I, I, P]),
     "rwkv7_a8w8_static_capacity_bytes": (L, []),
     "rwkv7_a8w8_linear_static": (I, [P] * 6 + [I, I, I, I, P]),
 }

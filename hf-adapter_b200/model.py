@@ -31,6 +31,7 @@ from . import norm_mix as _nm
 from . import packing as _pk
 from . import prep as _prep
 from . import recurrent as _rec
+from . import sampling as _smp
 from . import sharding as _sh
 from ._util import capture
 from .cache import NativeRWKV7Cache
@@ -195,9 +196,13 @@ def _causal_lm_output(logits, cache):
 
 def sample_next_token(logits, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, generator=None):
     """One token per row of ``logits [B,V]`` from the temperature-scaled distribution restricted to the ``top_k`` most
-    likely tokens and to the smallest set whose probability reaches ``top_p`` (the most likely token always stays)."""
+    likely tokens and to the smallest set whose probability reaches ``top_p`` (the most likely token always stays).  On the GPU
+    this is one launch (``sampling.sample_tokens``) on the variates that a multinomial draw takes from ``generator``."""
     if temperature <= 0:
         return logits.argmax(-1)
+    if logits.is_cuda and logits.dim() == 2 and logits.dtype in (torch.float16, torch.bfloat16, torch.float32):
+        noise = torch.empty(logits.shape, device=logits.device, dtype=torch.float32).exponential_(1.0, generator=generator)
+        return _smp.sample_tokens(logits, noise, temperature=float(temperature), top_k=int(top_k or 0), top_p=float(top_p))
     z = logits.float() / float(temperature)
     if top_k and 0 < int(top_k) < z.shape[-1]:
         kth = torch.topk(z, int(top_k), dim=-1).values[:, -1:]
@@ -612,11 +617,17 @@ class RWKV7ForCausalLM(nn.Module):
     @torch.no_grad()
     def generate(self, input_ids=None, attention_mask=None, max_new_tokens: int = 16, do_sample: bool = False,
                  temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, eos_token_id=None, pad_token_id: int = 0,
-                 use_graph: bool = True, generator=None, inputs=None, **_):
+                 use_graph: bool = True, generator=None, inputs=None, min_p: float = 0.0, repetition_penalty=1.0, presence_penalty=0.0,
+                 frequency_penalty=0.0, logit_bias=None, allowed_tokens=None, **_):
         """Prefill, then one decode step per new token; returns ``[B, T + new]`` ids.  Greedy by default (the head's
-        arg-max runs inside the decode graph); ``do_sample`` draws from the temperature / top-k / top-p filtered
+        arg-max runs inside the decode graph); ``do_sample`` draws from the temperature / top-k / top-p / min-p filtered
         distribution on the device.  A left-padded batch passes its ``attention_mask``: padded positions leave the
-        state untouched.  Sequences that produced ``eos_token_id`` are filled with ``pad_token_id``."""
+        state untouched.  Sequences that produced ``eos_token_id`` are filled with ``pad_token_id``.
+
+        ``repetition_penalty``, ``presence_penalty``, ``frequency_penalty`` (numbers or vectors ``[B]``), ``logit_bias`` and
+        ``allowed_tokens`` are the rules of ``process_logits``, applied in the launch that picks the token; ``allowed_tokens``
+        may be a function of the new tokens so far (``[B, n]``) that returns the words of the next step, or None.  A sequence
+        that no token is allowed for ends there."""
         if input_ids is None:
             input_ids = inputs
         if input_ids.dim() == 1:
@@ -631,23 +642,49 @@ class RWKV7ForCausalLM(nn.Module):
         if eos_token_id is not None:
             eos = torch.as_tensor([eos_token_id] if isinstance(eos_token_id, int) else list(eos_token_id), device=input_ids.device)
         done = torch.zeros(B, dtype=torch.bool, device=input_ids.device)
+        penalties = any(isinstance(v, torch.Tensor) or v != off
+                        for v, off in ((repetition_penalty, 1.0), (presence_penalty, 0.0), (frequency_penalty, 0.0)))
+        rules = {}
+        if penalties:
+            T = int(input_ids.shape[1])
+            history = torch.full((B, T + n_new), -1, device=input_ids.device, dtype=torch.int64)
+            history[:, :T] = input_ids
+            if attention_mask is not None:
+                history[:, :T].masked_fill_(attention_mask.to(input_ids.device).view(B, -1)[:, -T:] == 0, -1)
+            length = torch.full((B,), T, device=input_ids.device, dtype=torch.int32)
+            rules.update(tokens=history, lengths=length, prompt_lengths=length.clone(), repetition_penalty=repetition_penalty,
+                         presence_penalty=presence_penalty, frequency_penalty=frequency_penalty)
+        if logit_bias is not None:
+            rules["bias"] = logit_bias
+        picks = do_sample or penalties or logit_bias is not None or allowed_tokens is not None  # from the logits of every step
         toks = []
         for step in range(n_new):
             if step:
-                if do_sample:
+                if picks:
                     logits = self.rwkv7_forward_token(tok, cache, use_graph=use_graph)
                 else:
                     logits = None
                     tok = self.rwkv7_forward_token(tok, cache, use_graph=use_graph, return_tokens=True)
-            if do_sample:
-                tok = sample_next_token(logits, temperature=temperature, top_k=top_k, top_p=top_p, generator=generator)
+            if picks:
+                if allowed_tokens is not None:
+                    rules["allowed"] = (allowed_tokens(torch.cat(toks, 1) if toks else input_ids[:, :0]) if callable(allowed_tokens)
+                                        else allowed_tokens)
+                noise = None
+                if do_sample and temperature > 0:
+                    noise = torch.empty(logits.shape, device=logits.device, dtype=torch.float32).exponential_(1.0, generator=generator)
+                tok = _smp.sample_tokens(logits, noise, temperature=temperature, top_k=top_k or 0, top_p=top_p, min_p=min_p, **rules)
             elif logits is not None:
                 tok = logits.argmax(-1)
-            if eos is not None:
+            if eos is not None or allowed_tokens is not None:
+                done = done | (tok < 0)
                 tok = torch.where(done, torch.full_like(tok, int(pad_token_id)), tok)
+            if eos is not None:
                 done = done | torch.isin(tok, eos)
             toks.append(tok[:, None])
-            if eos is not None and step + 1 < n_new and bool(done.all()):
+            if penalties:
+                history[:, T + step] = tok
+                length += 1
+            if (eos is not None or allowed_tokens is not None) and step + 1 < n_new and bool(done.all()):
                 break
         return torch.cat([input_ids] + toks, dim=1)
 

@@ -488,6 +488,43 @@ int rwkv7_fp4_linear(const void* x, int64_t ldx, const void* w_packed, const voi
                      const void* bias, const void* residual, void* y, void* workspace, int64_t workspace_bytes, int M, int K, int N,
                      int epilogue, int format, int dtype, void* stream);
 
+/* ---- from logits to the next token (no counterpart in the reference, whose sampling is tensor code) ----
+ * Rules on the logits of a row, in fp32: with c = how often token v occurs in tokens[prompt_length, length) and seen = whether it
+ * occurs in tokens[0, length),
+ *   seen: z > 0 ? z / repetition : z * repetition;  z - frequency * c - presence * (c > 0) + bias[v];  -inf where not allowed.
+ * Every field may be NULL / 0 except the values that stand in for a NULL vector (repetition 1, the others 0 change nothing). */
+typedef struct {
+    const void* tokens;             /* [B, history], tokens_ld apart, int64 if tokens_i64 else int32; ids outside the vocabulary are skipped */
+    int64_t tokens_ld;
+    const int32_t* lengths;         /* [B]; NULL: history */
+    const int32_t* prompt_lengths;  /* [B]; NULL: 0 */
+    const float *repetition, *presence, *frequency; /* [B]; NULL: the value below */
+    const float* bias;              /* rows bias_ld apart (0: one row for all) */
+    int64_t bias_ld;
+    const int32_t* allowed;         /* bit v % 32 of word v / 32; rows allowed_ld words apart (0: one row for all) */
+    int64_t allowed_ld;
+    int32_t history, tokens_i64;
+    float repetition_value, presence_value, frequency_value;
+} rwkv7_logit_rules;
+/* What a row is drawn from: a vector [B], or the value where that is NULL. */
+typedef struct {
+    const float *temperature, *top_p, *min_p;
+    const int32_t* top_k;
+    float temperature_value, top_p_value, min_p_value;
+    int32_t top_k_value;
+} rwkv7_draw_params;
+/* out = rules(logits), rounded to dtype; rows ld / out_ld elements apart, any alignment; out may be logits. */
+int rwkv7_process_logits(const void* logits, int64_t ld, const rwkv7_logit_rules* rules, void* out, int64_t out_ld, int B, int V, int dtype,
+                         void* stream);
+/* One token a row: rules, z / temperature, then with e = exp(z - max)
+ *   top-k (0 or >= V: off) keeps z >= the k-th largest; top-p (>= 1: off) keeps, in descending order and lowest index first, what has
+ *   less than top_p of the top-k survivors' mass before it (always the first); min-p keeps e >= min_p;
+ *   token = argmax of e / noise over what is kept, lowest index first; noise [B, V] holds Exp(1) variates.
+ * temperature <= 0, or noise NULL: argmax of z (and z is not divided).  NaN is never drawn, +inf counts as the largest finite
+ * number; a row without any token gives -1.  logprob (may be NULL): log of e / (sum of e over all tokens), -inf for -1. */
+int rwkv7_sample_tokens(const void* logits, int64_t ld, const rwkv7_logit_rules* rules, const rwkv7_draw_params* draw, const float* noise,
+                        int64_t noise_ld, long long* token, float* logprob, int B, int V, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
