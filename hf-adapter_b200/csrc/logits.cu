@@ -16,6 +16,8 @@
 // masses that are added by atomics are 64-bit fixed point (2^-40): results repeat bit for bit.
 #include <cooperative_groups.h>
 
+#include <cstddef>
+
 #include "umma.cuh"
 
 namespace cg = cooperative_groups;
@@ -24,30 +26,57 @@ namespace rwkv7 {
 namespace lg {
 constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int MAX_CLUSTER = 8;
-constexpr int BINS = 512;            // of a histogram
-constexpr float BIN_SCALE = 16.0f;   // first histogram: m - z in steps of 1/16, the last bin takes the rest
+constexpr int BINS = 1024;           // of a histogram
+constexpr float BIN_SCALE = 32.0f;   // first histogram: m - z in steps of 1/32, the last bin takes the rest
+constexpr int LIST = 1024;           // tokens that the short way sorts
 constexpr float MASS_UNIT = 1099511627776.0f;  // 2^40
+constexpr float FLOAT_MAX = 3.402823466e38f;
 
-struct Exchange {
+typedef unsigned long long u64;
+
+struct Part {  // what a CTA found, relative to its own largest value
     double sum;
-    float value, z;
-    int index;
+    float max, score, z;
+    int top, index;
+};
+struct Cut {
+    unsigned int key;  // values with down_key <= key are kept
+    int index;         // of values with exactly this key only tokens below this one
+    u64 mass;          // of what the key keeps (by count only)
+    bool found;
 };
 struct Shared {
-    unsigned int count[BINS];          // this CTA's histogram
-    unsigned long long mass[BINS];
-    unsigned int all_count[2][BINS];   // the cluster's: [0] the first level, [1] the refinements
-    unsigned long long all_mass[2][BINS];
-    Exchange ex[3][MAX_CLUSTER];       // one for each use: nothing is written again while a CTA may still read it
-    Exchange warp_ex[WARPS];
-    unsigned int ties[MAX_CLUSTER];
-    unsigned int warp_ties[WARPS];
-    // crossing of a scan
-    int bin;
-    unsigned int above_count, bin_count;
-    unsigned long long above_mass, bin_mass, target;
-    int index_cut;
+    Part part[MAX_CLUSTER];           // first CTA: of every CTA
+    Part warp_part[WARPS];
+    double sum_of[MAX_CLUSTER];
+    u64 mass_of[2][2][MAX_CLUSTER];   // [top-k, top-p][of the tokens above the window, of those on the list]
+    u64 warp_mass[WARPS];
+    double warp_sum[WARPS];
+    Cut cut[2];
+    float max[MAX_CLUSTER], warp_max[WARPS], warp_est[WARPS];
+    int top[MAX_CLUSTER], warp_top[WARPS];
+    unsigned int warp_count[WARPS];
+    // from here on only where there are filters
+    unsigned int count[BINS];         // this CTA's histogram
+    unsigned int owned[BINS];         // the cluster's, for the bins that this CTA owns (the others' places stay unused)
+    unsigned int upto[BINS];          // the cluster's, summed from bin 0
+    unsigned int list_n[2];           // first CTA: places given out
+    unsigned int list_base, list_at;
+    int bin, window_first, window_last;
+    int place;
+    union {
+        u64 list[LIST];  // first CTA: down_key << 32 | token
+        struct {         // the descent
+            unsigned int count[BINS], all_count[BINS];
+            u64 mass[BINS], all_mass[BINS];
+            unsigned int ties[MAX_CLUSTER];
+            unsigned int above_count, bin_count;
+            u64 above_mass, bin_mass;
+            int index_cut;
+        } w;
+    };
 };
+constexpr int PICK_SHARED = (offsetof(Shared, count) + 15) / 16 * 16, FILTER_SHARED = (sizeof(Shared) + 15) / 16 * 16;
 }  // namespace lg
 
 struct Row {  // the rules of one row
@@ -71,15 +100,69 @@ __device__ __forceinline__ Row row_rules(const rwkv7_logit_rules& r, int64_t row
 }
 
 // word: the token's history; products and differences rounded one by one
-__device__ __forceinline__ float apply_rules(const Row& r, float z, unsigned int word, int v) {
+__device__ __forceinline__ float penalise(const Row& r, float z, unsigned int word) {
     if (word) {
         z = z > 0.0f ? z / r.repetition : z * r.repetition;
         const unsigned int c = word & 0x7fffffffu;
         z = __fsub_rn(__fsub_rn(z, __fmul_rn(r.frequency, (float)c)), c ? r.presence : 0.0f);
     }
-    if (r.bias) z = __fadd_rn(z, r.bias[v]);
-    if (r.allowed && !((r.allowed[v >> 5] >> (v & 31)) & 1)) z = -INFINITY;
     return z;
+}
+
+// One vector of VEC tokens from v0 on, of which those inside [0, V) count (the others become -inf); words: their history.
+template <typename T, int VEC, bool RULES>
+__device__ __forceinline__ void load_vector(const T* in, int v0, int V, const Row& r, const unsigned int* words, float (&z)[VEC]) {
+    if (v0 >= 0 && v0 + VEC <= V) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(in + v0);
+        const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[i] = to_f<T>(e[i]);
+        if constexpr (RULES) {
+            if (r.history) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) z[i] = penalise(r, z[i], words[i]);
+            }
+            if (r.bias) {
+                const float* b = r.bias + v0;
+                if ((reinterpret_cast<uintptr_t>(b) & 15) == 0) {
+#pragma unroll
+                    for (int h = 0; h < VEC; h += 4) {
+                        const float4 q = *reinterpret_cast<const float4*>(b + h);
+                        z[h] = __fadd_rn(z[h], q.x), z[h + 1] = __fadd_rn(z[h + 1], q.y);
+                        z[h + 2] = __fadd_rn(z[h + 2], q.z), z[h + 3] = __fadd_rn(z[h + 3], q.w);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) z[i] = __fadd_rn(z[i], b[i]);
+                }
+            }
+            if (r.allowed) {
+                const int at = v0 >> 5, sh = v0 & 31;
+                unsigned int bits = (unsigned int)r.allowed[at] >> sh;
+                if (sh > 32 - VEC) bits |= (unsigned int)r.allowed[at + 1] << (32 - sh);  // (the vector's last token is in the next word)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (!((bits >> i) & 1)) z[i] = -INFINITY;
+            }
+        }
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < VEC; ++i) {
+            const int v = v0 + i;
+            float x = -INFINITY;
+            if (v >= 0 && v < V) {
+                x = to_f<T>(in[v]);
+                if constexpr (RULES) {
+                    if (r.history) x = penalise(r, x, words[i]);
+                    if (r.bias) x = __fadd_rn(x, r.bias[v]);
+                    if (r.allowed && !((r.allowed[v >> 5] >> (v & 31)) & 1)) x = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < VEC; ++k)
+                if (k == i) z[k] = x;  // (no indexed registers)
+        }
+    }
 }
 
 // counts the history's tokens in [first, first + n) into words[0, n); ids outside the vocabulary fall outside every slice
@@ -119,63 +202,23 @@ __global__ void __launch_bounds__(256) process_logits_kernel(const T* logits, in
     for (int j = threadIdx.x * VEC; j < slice; j += blockDim.x * VEC) {
         const int v0 = first + j;
         if (v0 >= V) break;
-        if (v0 >= 0 && v0 + VEC <= V) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(in + v0);
-            const T* e = reinterpret_cast<const T*>(&raw);
-            alignas(16) T res[VEC];
+        float z[VEC];
+        load_vector<T, VEC, true>(in, v0, V, r, words + j, z);
+        alignas(16) T res[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) res[i] = from_f<T>(apply_rules(r, to_f<T>(e[i]), r.history ? words[j + i] : 0u, v0 + i));
-            if (vec_out) {
-                *reinterpret_cast<uint4*>(o + v0) = *reinterpret_cast<const uint4*>(res);
-            } else {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) o[v0 + i] = res[i];
-            }
+        for (int i = 0; i < VEC; ++i) res[i] = from_f<T>(z[i]);
+        if (vec_out && v0 >= 0 && v0 + VEC <= V) {
+            *reinterpret_cast<uint4*>(o + v0) = *reinterpret_cast<const uint4*>(res);
         } else {
+#pragma unroll
             for (int i = 0; i < VEC; ++i)
-                if (v0 + i >= 0 && v0 + i < V) o[v0 + i] = from_f<T>(apply_rules(r, to_f<T>(in[v0 + i]), r.history ? words[j + i] : 0u, v0 + i));
+                if (v0 + i >= 0 && v0 + i < V) o[v0 + i] = res[i];
         }
     }
 }
 
 // ---------------------------------------------------------------- the draw
 __device__ __forceinline__ bool better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
-
-// the block's best (value, lowest index first) with its z, and the block's sum in warp order; valid in every thread
-__device__ __forceinline__ lg::Exchange block_best(lg::Exchange x, lg::Shared& s) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float v = __shfl_xor_sync(0xffffffffu, x.value, o), z = __shfl_xor_sync(0xffffffffu, x.z, o);
-        const int i = __shfl_xor_sync(0xffffffffu, x.index, o);
-        x.sum += __shfl_xor_sync(0xffffffffu, x.sum, o);
-        if (better(v, i, x.value, x.index)) x.value = v, x.index = i, x.z = z;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s.warp_ex[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = s.warp_ex[0];
-    for (int w = 1; w < lg::WARPS; ++w) {
-        const lg::Exchange y = s.warp_ex[w];
-        x.sum += y.sum;
-        if (better(y.value, y.index, x.value, x.index)) x.value = y.value, x.index = y.index, x.z = y.z;
-    }
-    return x;
-}
-
-// the cluster's, in rank order; `slot` is used once a row
-__device__ __forceinline__ lg::Exchange cluster_best(lg::Exchange x, lg::Shared& s, int slot, cg::cluster_group& cl) {
-    x = block_best(x, s);
-    const int C = cl.num_blocks(), rank = cl.block_rank();
-    if ((int)threadIdx.x < C) cl.map_shared_rank(&s, threadIdx.x)->ex[slot][rank] = x;
-    cl.sync();
-    x = s.ex[slot][0];
-    for (int c = 1; c < C; ++c) {
-        const lg::Exchange y = s.ex[slot][c];
-        x.sum += y.sum;
-        if (better(y.value, y.index, x.value, x.index)) x.value = y.value, x.index = y.index, x.z = y.z;
-    }
-    return x;
-}
 
 __device__ __forceinline__ int linear_bin(float m, float z) {
     const float d = (m - z) * lg::BIN_SCALE;
@@ -190,9 +233,9 @@ __device__ __forceinline__ float key_value(unsigned int k) { return __uint_as_fl
 // the last key of bins 0 .. bin: linear_bin rises with the key, so a bisection between keys on both sides of the edge (the
 // bin's rounded edge is off by less than 2^-22 of the operands) finds it exactly
 __device__ __forceinline__ unsigned int last_key(float m, int bin) {
-    if (bin == lg::BINS - 1) return down_key(-3.402823466e38f);
+    if (bin == lg::BINS - 1) return down_key(-lg::FLOAT_MAX);
     const float edge = m - (float)(bin + 1) / lg::BIN_SCALE, slack = (fabsf(m) + 64.0f) * 1e-6f;
-    unsigned int lo = down_key(fminf(m, edge + slack)), hi = down_key(fmaxf(edge - slack, -3.402823466e38f));
+    unsigned int lo = down_key(fminf(m, edge + slack)), hi = down_key(fmaxf(edge - slack, -lg::FLOAT_MAX));
     while (lo < hi) {
         const unsigned int mid = lo + (hi - lo + 1) / 2;
         if (linear_bin(m, key_value(mid)) <= bin) lo = mid;
@@ -200,92 +243,145 @@ __device__ __forceinline__ unsigned int last_key(float m, int bin) {
     }
     return lo;
 }
-__device__ __forceinline__ unsigned long long fixed_mass(float e) { return __float2ull_rn(e * lg::MASS_UNIT); }
+__device__ __forceinline__ lg::u64 fixed_mass(float e) { return __float2ull_rn(e * lg::MASS_UNIT); }
+__device__ __forceinline__ lg::u64 share_of(double share, double mass) {
+    const double want = ceil(share * mass);
+    return want < 1.0 ? 1ull : (lg::u64)want;
+}
 
-// the cluster's histogram of `bin_of(z)` (negative: not counted) into all_count / all_mass[level] of every CTA
+// A slice is walked in its own vectors of VEC places by the thread that loaded them; `f(place, z)` for every token that is there.
+template <int VEC, typename F>
+__device__ __forceinline__ void each_token(const float* zs, int slice, F f) {
+    for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
+#pragma unroll
+        for (int h = 0; h < VEC; h += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(zs + j + h);
+            const float z[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (z[i] != -INFINITY) f(j + h + i, z[i]);
+        }
+    }
+}
+
+// log of a sum that is at least 1
+__device__ __forceinline__ float log_sum(double sum) { return log1pf((float)(sum - 1.0)); }
+
+__device__ __forceinline__ double warp_add(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ lg::u64 warp_add(lg::u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ void warp_best(float& v, int& i, float& z) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float w = __shfl_xor_sync(0xffffffffu, v, o), y = __shfl_xor_sync(0xffffffffu, z, o);
+        const int j = __shfl_xor_sync(0xffffffffu, i, o);
+        if (better(w, j, v, i)) v = w, i = j, z = y;
+    }
+}
+// the same value over the block, in every thread; `at` holds a place a warp and is not in use
+template <typename V> __device__ __forceinline__ V block_add(V v, V* at) {
+    v = warp_add(v);
+    if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    v = lane < lg::WARPS ? at[lane] : V(0);
+    v = warp_add(v);
+    __syncthreads();
+    return v;
+}
+// block maximum (lowest index first), in every thread
+__device__ __forceinline__ void block_max_index(float& v, int& i, lg::Shared& s) {
+    float none = 0.0f;
+    warp_best(v, i, none);
+    if ((threadIdx.x & 31) == 0) s.warp_max[threadIdx.x >> 5] = v, s.warp_top[threadIdx.x >> 5] = i;
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    v = s.warp_max[lane % lg::WARPS], i = s.warp_top[lane % lg::WARPS];
+    warp_best(v, i, none);
+}
+// the CTA's sum and best score (all threads' values relative to one maximum); valid in warp 0
+__device__ __forceinline__ lg::Part block_part(lg::Part x, lg::Shared& s) {
+    x.sum = warp_add(x.sum);
+    warp_best(x.score, x.index, x.z);
+    if ((threadIdx.x & 31) == 0) s.warp_part[threadIdx.x >> 5] = x;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        x = s.warp_part[threadIdx.x % lg::WARPS];
+        if (threadIdx.x >= lg::WARPS) x.sum = 0.0, x.score = -1.0f, x.index = 0x7fffffff;
+        x.sum = warp_add(x.sum);
+        warp_best(x.score, x.index, x.z);
+    }
+    return x;
+}
+
+// ------------------------------ the descent: any number of equal or neighbouring values at a cut
+// the cluster's histogram of counts and masses over `bin_of(z)` (negative: not counted) into every CTA
 template <typename F>
-__device__ __forceinline__ void histogram(const float* zs, int slice, float m, lg::Shared& s, int level, cg::cluster_group& cl, F bin_of) {
-    for (int b = threadIdx.x; b < lg::BINS; b += lg::THREADS) s.count[b] = 0, s.mass[b] = 0;
+__device__ __forceinline__ void histogram(const float* zs, int slice, float m, lg::Shared& s, cg::cluster_group& cl, F bin_of) {
+    for (int b = threadIdx.x; b < lg::BINS; b += lg::THREADS) s.w.count[b] = 0, s.w.mass[b] = 0;
     __syncthreads();
     for (int j = threadIdx.x; j < slice; j += lg::THREADS) {
         const float z = zs[j];
         if (z == -INFINITY) continue;
         const int b = bin_of(z);
         if (b >= 0) {
-            atomicAdd(&s.count[b], 1u);
-            atomicAdd(&s.mass[b], fixed_mass(expf(z - m)));
+            atomicAdd(&s.w.count[b], 1u);
+            atomicAdd(&s.w.mass[b], fixed_mass(expf(z - m)));
         }
     }
     cl.sync();
     const int C = cl.num_blocks(), rank = cl.block_rank(), per = lg::BINS / C;
     for (int b = rank * per + threadIdx.x; b < (rank + 1) * per; b += lg::THREADS) {
         unsigned int n = 0;
-        unsigned long long q = 0;
+        lg::u64 q = 0;
         for (int c = 0; c < C; ++c) {
             lg::Shared* o = cl.map_shared_rank(&s, c);
-            n += o->count[b], q += o->mass[b];
+            n += o->w.count[b], q += o->w.mass[b];
         }
         for (int c = 0; c < C; ++c) {
             lg::Shared* o = cl.map_shared_rank(&s, c);
-            o->all_count[level][b] = n, o->all_mass[level][b] = q;
+            o->w.all_count[b] = n, o->w.all_mass[b] = q;
         }
     }
     cl.sync();
 }
 
-__device__ __forceinline__ unsigned long long share_of(double share, unsigned long long mass) {
-    const double want = ceil(share * (double)mass);
-    return want < 1.0 ? 1ull : (unsigned long long)want;
-}
-
-// first bin at which count (or mass) above the range plus that of bins 0 .. b reaches the target; results in s (bin = -1: none).
-// share > 0: the target is that share of all the mass, rounded up.
-__device__ __forceinline__ void find_crossing(lg::Shared& s, int level, bool by_mass, unsigned long long target, double share,
-                                              unsigned int base_count, unsigned long long base_mass) {
+// first bin at which count (or mass) above the range plus that of bins 0 .. b reaches the target; results in s.w (bin = -1: none)
+__device__ __forceinline__ void find_crossing(lg::Shared& s, bool by_mass, lg::u64 target, unsigned int base_count, lg::u64 base_mass) {
+    static_assert(lg::BINS == 2 * lg::THREADS, "two bins a thread");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = 2 * threadIdx.x;
+    const unsigned int n0 = s.w.all_count[b], n1 = s.w.all_count[b + 1];
+    const lg::u64 q0 = s.w.all_mass[b], q1 = s.w.all_mass[b + 1];
+    unsigned int n = n0 + n1;
+    lg::u64 q = q0 + q1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned int tn = __shfl_up_sync(0xffffffffu, n, o);
+        const lg::u64 tq = __shfl_up_sync(0xffffffffu, q, o);
+        if (lane >= o) n += tn, q += tq;
+    }
+    if (lane == 31) s.warp_count[warp] = n, s.warp_mass[warp] = q;
+    if (threadIdx.x == 0) s.bin = -1;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        constexpr int PER = lg::BINS / 32;
-        const int lane = threadIdx.x;
-        unsigned int n = 0;
-        unsigned long long q = 0;
-        for (int i = 0; i < PER; ++i) n += s.all_count[level][lane * PER + i], q += s.all_mass[level][lane * PER + i];
-        unsigned int cn = n;
-        unsigned long long cq = q;
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned int tn = __shfl_up_sync(0xffffffffu, cn, o);
-            const unsigned long long tq = __shfl_up_sync(0xffffffffu, cq, o);
-            if (lane >= o) cn += tn, cq += tq;
-        }
-        if (share > 0.0) target = share_of(share, __shfl_sync(0xffffffffu, cq, 31));
-        if (lane == 0) s.target = target;
-        cn += base_count, cq += base_mass;
-        const bool reached = (by_mass ? cq : (unsigned long long)cn) >= target;
-        const unsigned int who = __ballot_sync(0xffffffffu, reached);
-        if (who == 0) {
-            if (lane == 0) s.bin = -1;
-        } else if (lane == __ffs(who) - 1) {
-            unsigned int an = cn - n;
-            unsigned long long aq = cq - q;
-            for (int i = 0; i < PER; ++i) {
-                const int b = lane * PER + i;
-                const unsigned int bn = s.all_count[level][b];
-                const unsigned long long bq = s.all_mass[level][b];
-                if ((by_mass ? aq + bq : (unsigned long long)(an + bn)) >= target) {
-                    s.bin = b, s.bin_count = bn, s.bin_mass = bq, s.above_count = an, s.above_mass = aq;
-                    break;
-                }
-                an += bn, aq += bq;
-            }
-        }
+    unsigned int an = base_count + n - n0 - n1;  // before this thread's bins
+    lg::u64 aq = base_mass + q - q0 - q1;
+    for (int w = 0; w < warp; ++w) an += s.warp_count[w], aq += s.warp_mass[w];
+    const bool before = (by_mass ? aq : (lg::u64)an) >= target, first = (by_mass ? aq + q0 : (lg::u64)(an + n0)) >= target;
+    const bool second = (by_mass ? aq + q0 + q1 : (lg::u64)(an + n0 + n1)) >= target;
+    if (!before && second) {
+        s.bin = first ? b : b + 1;
+        s.w.bin_count = first ? n0 : n1, s.w.bin_mass = first ? q0 : q1;
+        s.w.above_count = first ? an : an + n0, s.w.above_mass = first ? aq : aq + q0;
     }
     __syncthreads();
 }
-
-struct Cut {
-    unsigned int key;            // values with down_key <= key are kept
-    int index;                   // of values with exactly this key only tokens below this one
-    unsigned long long mass;     // of what the key keeps
-};
 
 // Equal values at the cut, of which `need` are kept, lowest index first: the first token of this slice that is not kept.
 __device__ __forceinline__ int tie_cut(const float* zs, int slice, int first, unsigned int key, unsigned int need, lg::Shared& s,
@@ -299,148 +395,494 @@ __device__ __forceinline__ int tie_cut(const float* zs, int slice, int first, un
         const unsigned int t = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += t;
     }
-    if (lane == 31) s.warp_ties[warp] = upto;
-    if (threadIdx.x == 0) s.index_cut = 0x7fffffff;
+    if (lane == 31) s.warp_count[warp] = upto;
+    if (threadIdx.x == 0) s.w.index_cut = 0x7fffffff;
     __syncthreads();
     unsigned int total = 0, at = upto - mine;
     for (int w = 0; w < lg::WARPS; ++w) {
-        if (w < warp) at += s.warp_ties[w];
-        total += s.warp_ties[w];
+        if (w < warp) at += s.warp_count[w];
+        total += s.warp_count[w];
     }
     const int C = cl.num_blocks(), rank = cl.block_rank();
-    if ((int)threadIdx.x < C) cl.map_shared_rank(&s, threadIdx.x)->ties[rank] = total;
+    if ((int)threadIdx.x < C) cl.map_shared_rank(&s, threadIdx.x)->w.ties[rank] = total;
     cl.sync();
     unsigned int ahead = 0;
-    for (int c = 0; c < rank; ++c) ahead += s.ties[c];
+    for (int c = 0; c < rank; ++c) ahead += s.w.ties[c];
     if (ahead >= need) return 0;  // an earlier slice has them all
     at += ahead;
     for (int j = j0; j < j1; ++j)
-        if (zs[j] != -INFINITY && down_key(zs[j]) == key && at++ == need) s.index_cut = first + j;
+        if (zs[j] != -INFINITY && down_key(zs[j]) == key && at++ == need) s.w.index_cut = first + j;
     __syncthreads();
-    return s.index_cut;
+    return s.w.index_cut;
 }
 
-// The key at which the descending order reaches `target` tokens (or mass, or a share of all of it), from the first level's
-// histogram down.  A range of keys that is kept as a whole ends the search; its last key is the cut.
-__device__ __forceinline__ Cut find_cut(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, bool by_mass,
-                                        unsigned long long target, double share) {
-    find_crossing(s, 0, by_mass, target, share, 0, 0);
-    if (s.bin < 0) return Cut{0xffffffffu, 0x7fffffff, 0};  // (only by count: fewer tokens than k)
-    target = s.target;
+// The key at which the descending order reaches `target` tokens (or mass).  A range of keys that is kept as a whole ends the
+// search; its last key is the cut.
+__device__ __noinline__ lg::Cut descend(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, bool by_mass,
+                                           lg::u64 target) {
+    using lg::Cut;
+    histogram(zs, slice, m, s, cl, [&](float z) { return linear_bin(m, z); });
+    find_crossing(s, by_mass, target, 0, 0);
+    if (s.bin < 0) return Cut{0xffffffffu, 0x7fffffff, 0, false};  // (only by count: fewer tokens than k)
     unsigned int lo = s.bin == 0 ? down_key(m) : last_key(m, s.bin - 1) + 1, hi = last_key(m, s.bin);
-    for (int level = 0;; ++level) {  // (32 bits of key in steps of 9: four refinements at most)
-        const unsigned int above_count = s.above_count, count = s.bin_count;
-        const unsigned long long above_mass = s.above_mass, mass = s.bin_mass;
+    for (int level = 0;; ++level) {  // (32 bits of key in steps of 10: four refinements at most)
+        const unsigned int above_count = s.w.above_count, count = s.w.bin_count;
+        const lg::u64 above_mass = s.w.above_mass, mass = s.w.bin_mass;
         // a single token, or (by count) all of them: the range is kept as a whole
         if (count == 1 || lo == hi || (!by_mass && above_count + count == target) || level == 4) {
-            Cut cut{hi, 0x7fffffff, above_mass + mass};
+            Cut cut{hi, 0x7fffffff, above_mass + mass, true};
             if (by_mass && count > 1) {
-                const unsigned long long each = mass / count, need = (target - above_mass + each - 1) / each;
+                const lg::u64 each = mass / count, need = (target - above_mass + each - 1) / each;
                 if (need < count) cut.index = tie_cut(zs, slice, first, hi, (unsigned int)need, s, cl);
             }
             return cut;
         }
-        const int bits = 32 - __clz(hi - lo), shift = bits > 9 ? bits - 9 : 0;
-        histogram(zs, slice, m, s, 1, cl, [&](float z) {
+        const int bits = 32 - __clz(hi - lo), shift = bits > 10 ? bits - 10 : 0;
+        histogram(zs, slice, m, s, cl, [&](float z) {
             const unsigned int k = down_key(z);
             return k >= lo && k <= hi ? (int)((k - lo) >> shift) : -1;
         });
-        find_crossing(s, 1, by_mass, target, 0.0, above_count, above_mass);
-        if (s.bin < 0) return Cut{hi, 0x7fffffff, above_mass + mass};
+        find_crossing(s, by_mass, target, above_count, above_mass);
+        if (s.bin < 0) return Cut{hi, 0x7fffffff, above_mass + mass, true};
         lo += (unsigned int)s.bin << shift;
         const unsigned int end = lo + ((1u << shift) - 1);
         hi = end < hi ? end : hi;
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(lg::THREADS, 1) sample_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
-                                                             const rwkv7_draw_params draw, const float* __restrict__ noise, int64_t noise_ld,
-                                                             long long* __restrict__ token, float* __restrict__ logprob, int V, int slice) {
+// ------------------------------ a window of bins around the cut, sorted
+// Which bins go on the list of the first CTA: from the first bin if what may be kept fits it, else a window around the cut; in
+// s.window_first, s.window_last (first > last: not even the cut's bin fits).  The cut's bin is known by count (k > 0), or
+// estimated: a bin's mass is taken as its count times e of its middle (1.6 % off at most), and two bins on either side allow
+// for that; the exact masses decide later.
+__device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, float want) {
+    static_assert(lg::BINS == 2 * lg::THREADS, "two bins a thread");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = 2 * threadIdx.x;
+    if (threadIdx.x == 0) s.bin = lg::BINS - 1;
+    __syncthreads();
+    if (k) {
+        const unsigned int before = b ? s.upto[b - 1] : 0;
+        if (before < k && s.upto[b + 1] >= k) s.bin = s.upto[b] >= k ? b : b + 1;
+    } else {
+        const unsigned int n0 = s.upto[b] - (b ? s.upto[b - 1] : 0), n1 = s.upto[b + 1] - s.upto[b];
+        const float middle = expf(-((float)b + 0.5f) / lg::BIN_SCALE), q0 = (float)n0 * middle;
+        const float q1 = (float)n1 * middle * 0.969233234f;  // e^(-1/32)
+        float q = q0 + q1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float t = __shfl_up_sync(0xffffffffu, q, o);
+            if (lane >= o) q += t;
+        }
+        if (lane == 31) s.warp_est[warp] = q;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) q += s.warp_est[w];
+        const bool before = q - q0 - q1 >= want;
+        // (rounding may let two neighbours claim the crossing, or none: the last bin then)
+        if (!before && q >= want) s.bin = q - q1 >= want ? b : b + 1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int bin = s.bin, wide = k ? bin : min(bin + 2, lg::BINS - 1);
+        int first = 0, last = wide;
+        if (s.upto[wide] > lg::LIST) {
+            first = k ? bin : max(bin - 2, 0);
+            auto tokens = [&] { return s.upto[last] - (first ? s.upto[first - 1] : 0); };
+            while (first <= last && tokens() > lg::LIST) {
+                if (last > bin) --last;
+                else ++first;
+            }
+        }
+        s.window_first = first, s.window_last = last;
+    }
+    __syncthreads();
+}
+
+// Every token of the window, no key beyond `limit`, to the first CTA's list; the masses (if asked for) of it and of what lies
+// above to every CTA.  Ends with a cluster barrier.
+template <int VEC>
+__device__ __forceinline__ void gather(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, int stage,
+                                       unsigned int limit, bool masses) {
+    using lg::u64;
+    const int w0 = s.window_first, w1 = s.window_last, C = cl.num_blocks(), rank = cl.block_rank();
+    u64 mine = 0;  // (tokens of the window in this slice; some may lie beyond the limit)
+    for (int b = w0 + threadIdx.x; b <= w1; b += lg::THREADS) mine += s.count[b];
+    mine = block_add(mine, s.warp_mass);
+    lg::Shared* head = cl.map_shared_rank(&s, 0);
+    if (threadIdx.x == 0) s.list_base = mine ? atomicAdd(&head->list_n[stage], (unsigned int)mine) : 0, s.list_at = 0;
+    __syncthreads();
+    u64 above = 0, listed = 0;
+    if (mine || (masses && w0))
+        each_token<VEC>(zs, slice, [&](int j, float z) {
+            const int b = linear_bin(m, z);
+            if (b > w1) return;
+            const u64 e = masses ? fixed_mass(expf(z - m)) : 0;
+            if (b < w0) {
+                above += e;
+                return;
+            }
+            const unsigned int key = down_key(z);
+            const bool in = key <= limit;
+            if (in) listed += e;
+            head->list[s.list_base + atomicAdd(&s.list_at, 1u)] = in ? (u64)key << 32 | (unsigned int)(first + j) : ~0ull;
+        });
+    if (masses) {
+        above = block_add(above, s.warp_mass), listed = block_add(listed, s.warp_mass);
+        if ((int)threadIdx.x < C) {
+            lg::Shared* o = cl.map_shared_rank(&s, threadIdx.x);
+            o->mass_of[stage][0][rank] = above, o->mass_of[stage][1][rank] = listed;
+        }
+    }
+    cl.sync();
+}
+
+// list[0, n) ascending, n at most LIST; what pads it to a power of two is the largest key
+__device__ __forceinline__ void sort_list(lg::u64* list, int n) {
+    int size = 32;
+    while (size < n) size *= 2;
+    for (int i = n + threadIdx.x; i < size; i += lg::THREADS) list[i] = ~0ull;
+    __syncthreads();
+    for (int span = 2; span <= size; span *= 2)
+        for (int d = span / 2; d > 0; d /= 2) {
+            for (int t = threadIdx.x; t < size / 2; t += lg::THREADS) {
+                const int i = 2 * t - (t & (d - 1));
+                const lg::u64 a = list[i], b = list[i + d];
+                if ((a > b) == ((i & span) == 0)) list[i] = b, list[i + d] = a;
+            }
+            __syncthreads();
+        }
+}
+
+// what the two places of this thread on the sorted list hold, and the mass before them
+struct Places {
+    float z[2], e[2];
+    lg::u64 w[2], before, total;
+};
+__device__ __forceinline__ Places weigh_list(const lg::u64* list, int n, float m, lg::u64 above, lg::Shared& s) {
+    static_assert(lg::LIST == 2 * lg::THREADS, "two places a thread");
+    const int i0 = threadIdx.x * 2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Places o;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        o.z[i] = i0 + i < n ? key_value((unsigned int)(list[i0 + i] >> 32)) : -INFINITY;
+        o.e[i] = expf(o.z[i] - m), o.w[i] = fixed_mass(o.e[i]);
+    }
+    lg::u64 upto = o.w[0] + o.w[1];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const lg::u64 t = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += t;
+    }
+    if (lane == 31) s.warp_mass[warp] = upto;
+    __syncthreads();
+    o.before = above + upto - o.w[0] - o.w[1], o.total = above;
+    for (int w = 0; w < lg::WARPS; ++w) {
+        const lg::u64 t = s.warp_mass[w];
+        if (w < warp) o.before += t;
+        o.total += t;
+    }
+    __syncthreads();
+    return o;
+}
+// places of the sorted list that hold keys up to `key`
+__device__ __forceinline__ int places_upto(const lg::u64* list, int n, unsigned int key) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if ((unsigned int)(list[mid] >> 32) <= key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// e = exp(d) for the sums and races over all tokens: one ex2, off by 2^-22 and |d| 2^-23; what decides a cut by mass uses expf
+__device__ __forceinline__ float fast_exp(float d) { return __expf(d); }
+
+// The draw of one row, and which of its filters are on
+struct Draw {
+    float temperature, p, min_p;
+    int k;
+    bool greedy, by_k, by_p;
+};
+__device__ __forceinline__ Draw row_draw(const rwkv7_draw_params& d, bool noise, int64_t row, int V) {
+    Draw o;
+    o.temperature = noise ? param(d.temperature, d.temperature_value, row) : 0.0f;
+    o.greedy = !(o.temperature > 0.0f);
+    o.k = d.top_k ? d.top_k[row] : d.top_k_value;
+    o.p = param(d.top_p, d.top_p_value, row), o.min_p = param(d.min_p, d.min_p_value, row);
+    o.by_k = !o.greedy && o.k > 0 && o.k < V, o.by_p = !o.greedy && o.p < 1.0f;
+    return o;
+}
+
+// z / t for finite results below 1e37 as a product with 1 / t and one correction step (the correctly rounded quotient); the rest
+// (what is masked, NaN, out of range) on its own
+__device__ __forceinline__ float over_temperature(float x, float t, float inv) {
+    const float q = x * inv;
+    float z = fmaf(fmaf(-q, t, x), inv, q) + 0.0f;  // (-0 becomes 0)
+    if (!(fabsf(q) < 1e37f)) z = x > -INFINITY ? fminf(x / t, lg::FLOAT_MAX) : -INFINITY;  // (NaN compares false)
+    return z;
+}
+
+// This CTA's slice of a row, ruled and divided, to zs; its largest value with the first token that has it
+template <typename T, bool RULES>
+__device__ __forceinline__ void load_row(const T* in, int first, int V, int slice, const rwkv7_logit_rules& rules, int64_t row, const Draw& d,
+                                         float* zs, float& m, int& top) {
+    constexpr int VEC = 16 / sizeof(T);
+    Row r{};
+    if constexpr (RULES) {
+        r = row_rules(rules, row);
+        if (r.history) count_history(rules, row, first, slice, reinterpret_cast<unsigned int*>(zs));
+    }
+    const float t = d.greedy ? 1.0f : d.temperature, inv = __frcp_rn(t);
+    m = -INFINITY, top = 0x7fffffff;
+    for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
+        const int v0 = first + j;
+        float z[VEC];
+        load_vector<T, VEC, RULES>(in, v0, V, r, reinterpret_cast<unsigned int*>(zs) + j, z);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            z[i] = over_temperature(z[i], t, inv);
+            if (z[i] > m) m = z[i], top = v0 + i;
+        }
+#pragma unroll
+        for (int h = 0; h < VEC; h += 4) *reinterpret_cast<float4*>(zs + j + h) = make_float4(z[h], z[h + 1], z[h + 2], z[h + 3]);
+    }
+}
+
+// The largest value of the row, in every CTA of the cluster.  Ends with a cluster barrier.
+__device__ __forceinline__ void row_max(float& m, int& top, lg::Shared& s, cg::cluster_group& cl) {
+    const int C = cl.num_blocks(), rank = cl.block_rank();
+    if ((int)threadIdx.x < C) {
+        lg::Shared* o = cl.map_shared_rank(&s, threadIdx.x);
+        o->max[rank] = m, o->top[rank] = top;
+    }
+    cl.sync();
+    m = s.max[0], top = s.top[0];
+    for (int c = 1; c < C; ++c)
+        if (better(s.max[c], s.top[c], m, top)) m = s.max[c], top = s.top[c];
+}
+
+// Sum of exponentials and the race over this CTA's tokens that `keep(key, token, e)` lets in, and the row's answer from the parts
+template <int VEC, typename F>
+__device__ __forceinline__ void finish(const float* zs, int slice, int first, float m, int top, const Draw& d, const float* q, bool sums,
+                                       lg::Shared& s, cg::cluster_group& cl, long long* token, float* logprob, F keep) {
+    using lg::Part;
+    const int C = cl.num_blocks(), rank = cl.block_rank();
+    Part best{0.0, m, -1.0f, 0.0f, top, 0x7fffffff};
+    if ((sums || !d.greedy) && m != -INFINITY)
+        for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
+#pragma unroll
+            for (int h = 0; h < VEC; h += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
+                const float z[4] = {w.x, w.y, w.z, w.w};
+                float part = 0.0f;
+                int ones = 0;  // counted apart: a sure token's log-probability is all in the small terms
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = fast_exp(z[i] - m);
+                    if (e == 1.0f) ++ones;
+                    else part += e;
+                    const int v = first + j + h + i;
+                    if (!d.greedy && z[i] != -INFINITY && keep(z[i], v, e)) {
+                        const float score = __fdividef(e, q[v]);
+                        if (score > best.score) best.score = score, best.index = v, best.z = z[i];  // (tokens come in order)
+                    }
+                }
+                best.sum += (double)part + (double)ones;
+            }
+        }
+    best = block_part(best, s);
+    if (threadIdx.x == 0) cl.map_shared_rank(&s, 0)->part[rank] = best;
+    cl.sync();
+    if (rank == 0 && threadIdx.x < 32) {
+        Part x = s.part[threadIdx.x % C];
+        if ((int)threadIdx.x >= C) x = Part{0.0, -INFINITY, -1.0f, 0.0f, 0x7fffffff, 0x7fffffff};
+        float most = x.max, none = 0.0f;
+        int at = x.top;
+        warp_best(most, at, none);
+        const float f = x.max == -INFINITY ? 0.0f : expf(x.max - most);
+        const double sum = warp_add(x.sum * (double)f);
+        if (x.index != 0x7fffffff) x.score *= f;
+        warp_best(x.score, x.index, x.z);
+        if (threadIdx.x == 0) {
+            // (noise of NaN alone: the most likely token)
+            const bool empty = most == -INFINITY, drawn = !d.greedy && x.index != 0x7fffffff;
+            *token = empty ? -1 : drawn ? x.index : at;
+            if (logprob) *logprob = empty ? -INFINITY : ((drawn ? x.z : most) - most) - log_sum(sum);
+        }
+    }
+}
+
+// Rows without top-k and top-p
+template <typename T, bool RULES>
+__global__ void __launch_bounds__(lg::THREADS, 3) pick_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
+                                                              const rwkv7_draw_params draw, const float* __restrict__ noise, int64_t noise_ld,
+                                                              long long* __restrict__ token, float* __restrict__ logprob, int V, int slice) {
     using namespace lg;
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
-    float* zs = reinterpret_cast<float*>(smem + (sizeof(Shared) + 15) / 16 * 16);
+    float* zs = reinterpret_cast<float*>(smem + PICK_SHARED);
+    cg::cluster_group cl = cg::this_cluster();
+    constexpr int VEC = 16 / sizeof(T);
+    const int64_t row = blockIdx.x / cl.num_blocks();
+    const T* in = logits + row * ld;
+    const int first = cl.block_rank() * slice - (int)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % VEC);
+    cluster_arrive_relaxed();  // this CTA runs: the others may write into its shared memory
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const Draw d = row_draw(draw, noise != nullptr, row, V);
+    float m;
+    int top;
+    load_row<T, RULES>(in, first, V, slice, rules, row, d, zs, m, top);
+    block_max_index(m, top, s);
+    cluster_wait();
+    const float* q = noise + row * noise_ld;
+    float* lp = logprob ? logprob + row : nullptr;
+    const bool by_min = !d.greedy && d.min_p > 0.0f;  // the largest value of the row is needed first
+    if (by_min) row_max(m, top, s, cl);
+    const float least = by_min ? d.min_p : 0.0f;
+    finish<VEC>(zs, slice, first, m, top, d, q, lp != nullptr, s, cl, token + row, lp, [&](float, int, float e) { return e >= least; });
+}
+
+// Rows with top-k or top-p
+template <typename T, bool RULES>
+__global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
+                                                                const rwkv7_draw_params draw, const float* __restrict__ noise, int64_t noise_ld,
+                                                                long long* __restrict__ token, float* __restrict__ logprob, int V, int slice) {
+    using namespace lg;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Shared& s = *reinterpret_cast<Shared*>(smem);
+    float* zs = reinterpret_cast<float*>(smem + FILTER_SHARED);
     cg::cluster_group cl = cg::this_cluster();
     constexpr int VEC = 16 / sizeof(T);
     const int C = cl.num_blocks(), rank = cl.block_rank();
     const int64_t row = blockIdx.x / C;
     const T* in = logits + row * ld;
-    const int mis = (int)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % VEC);
-    const int first = rank * slice - mis;
-    const Row r = row_rules(rules, row);
-    const float temperature = noise ? param(draw.temperature, draw.temperature_value, row) : 0.0f;
-    const bool greedy = !(temperature > 0.0f);
-    const float divisor = greedy ? 1.0f : temperature;
-
+    const int first = rank * slice - (int)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % VEC);
+    if (threadIdx.x < 2) s.list_n[threadIdx.x] = 0;
+    for (int b = threadIdx.x; b < BINS; b += THREADS) s.count[b] = 0, s.owned[b] = 0;
     cluster_arrive_relaxed();  // this CTA runs: the others may write into its shared memory
-    if (r.history) count_history(rules, row, first, slice, reinterpret_cast<unsigned int*>(zs));
-    Exchange x{0.0, -INFINITY, 0.0f, 0x7fffffff};
-    for (int j = threadIdx.x * VEC; j < slice; j += THREADS * VEC) {
-        const int v0 = first + j;
-        const bool whole = v0 >= 0 && v0 + VEC <= V;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (whole) raw = *reinterpret_cast<const uint4*>(in + v0);
-        const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int v = v0 + i;
-            float z = -INFINITY;
-            if (v >= 0 && v < V) {
-                z = apply_rules(r, to_f<T>(whole ? e[i] : in[v]), r.history ? __float_as_uint(zs[j + i]) : 0u, v) / divisor;
-                z = z == z ? fminf(z, 3.402823466e38f) + 0.0f : -INFINITY;  // (-0 becomes 0)
-            }
-            zs[j + i] = z;
-            if (better(z, v, x.value, x.index)) x.value = z, x.index = v;
-        }
-    }
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const Draw d = row_draw(draw, noise != nullptr, row, V);
+    const int k = d.k;
+    const bool by_k = d.by_k, by_p = d.by_p;
+    const float* q = noise + row * noise_ld;
+    float m;
+    int top;
+    load_row<T, RULES>(in, first, V, slice, rules, row, d, zs, m, top);
+    block_max_index(m, top, s);
     cluster_wait();
-    x = cluster_best(x, s, 0, cl);
-    const float m = x.value;
-    const int top = x.index;
-    if (m == -INFINITY) {  // no token at all
-        if (rank == 0 && threadIdx.x == 0) {
-            token[row] = -1;
-            if (logprob) logprob[row] = -INFINITY;
+    row_max(m, top, s, cl);
+    Cut cut_k{0xffffffffu, 0x7fffffff, 0, false}, cut_p{0xffffffffu, 0x7fffffff, 0, false};
+    if ((by_k || by_p) && m != -INFINITY) {
+        // counts by distance from the largest value; every CTA sums up the bins it owns and reads the others' from their owners
+        double sum = 0.0;
+        each_token<VEC>(zs, slice, [&](int, float z) {
+            atomicAdd(&s.count[linear_bin(m, z)], 1u);
+            sum += (double)fast_exp(z - m);
+        });
+        sum = block_add(sum, s.warp_sum);  // (its barriers also end the counting)
+        const int per = BINS / C;
+        for (int b = threadIdx.x; b < BINS; b += THREADS)
+            if (s.count[b]) atomicAdd(&cl.map_shared_rank(&s, b / per)->owned[b], s.count[b]);
+        if ((int)threadIdx.x < C) cl.map_shared_rank(&s, threadIdx.x)->sum_of[rank] = sum;
+        cl.sync();
+        double all = 0.0;
+        for (int c = 0; c < C; ++c) all += s.sum_of[c];
+        {
+            const int b = 2 * threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+            const uint2 n = *reinterpret_cast<const uint2*>(&cl.map_shared_rank(&s, b / per)->owned[b]);
+            unsigned int c = n.x + n.y;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned int t = __shfl_up_sync(0xffffffffu, c, o);
+                if (lane >= o) c += t;
+            }
+            if (lane == 31) s.warp_count[warp] = c;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) c += s.warp_count[w];
+            s.upto[b] = c - n.y, s.upto[b + 1] = c;
+            __syncthreads();
         }
-        return;
-    }
-    Cut cut_k{0xffffffffu, 0x7fffffff, 0}, cut_p{0xffffffffu, 0x7fffffff, 0};
-    const float min_p = param(draw.min_p, draw.min_p_value, row);
-    if (!greedy) {
-        const int k = draw.top_k ? draw.top_k[row] : draw.top_k_value;
-        const float p = param(draw.top_p, draw.top_p_value, row);
-        const bool by_k = k > 0 && k < V, by_p = p < 1.0f;
-        if (by_k || by_p) {
-            histogram(zs, slice, m, s, 0, cl, [&](float z) { return linear_bin(m, z); });
-            if (by_k) cut_k = find_cut(zs, slice, first, m, s, cl, false, (unsigned long long)k, 0.0);
-            // of the mass that top-k keeps, or of all
-            const double share = p > 0.0f ? (double)p : 1e-300;
-            if (by_p) cut_p = find_cut(zs, slice, first, m, s, cl, true, share_of(share, cut_k.mass), cut_k.mass ? 0.0 : share);
+        const double share = d.p > 0.0f ? (double)d.p : 0.0;
+        u64 target_p = share_of(share * MASS_UNIT, all);
+#pragma unroll 1
+        for (int stage = by_k && (unsigned int)k < s.upto[BINS - 1] ? 0 : 1; stage < (by_p ? 2 : 1); ++stage) {
+            if (stage == 1 && cut_k.found) target_p = share_of(share, (double)cut_k.mass);
+            choose_window(s, stage == 0 ? (unsigned int)k : 0u, (float)((double)target_p / MASS_UNIT));
+            const int w0 = s.window_first, w1 = s.window_last;
+            bool done = false;
+            if (w0 <= w1) {
+                gather<VEC>(zs, slice, first, m, s, cl, stage, cut_k.key, by_p);
+                u64 above = 0, listed = 0;
+                for (int c = 0; by_p && c < C; ++c) above += s.mass_of[stage][0][c], listed += s.mass_of[stage][1][c];
+                // (by count the window is right; by mass the exact one has to agree, or everything is on the list)
+                const bool right = stage == 0 || (above < target_p && above + listed >= target_p) || (w0 == 0 && w1 == BINS - 1);
+                if (right && w0 == 0 && rank) return;  // the first CTA has all that may be kept
+                if (right && rank == 0) {
+                    const int n = (int)(s.upto[w1] - (w0 ? s.upto[w0 - 1] : 0));
+                    sort_list(s.list, n);
+                    const unsigned int above_count = w0 ? s.upto[w0 - 1] : 0;
+                    const unsigned int last = stage == 0 ? (unsigned int)(s.list[k - (int)above_count - 1] >> 32) : cut_k.key;
+                    const int kept = cut_k.found || stage == 0 ? places_upto(s.list, n, last) : n;
+                    const Places o = weigh_list(s.list, kept, m, above, s);
+                    const int i0 = threadIdx.x * 2;
+                    if (w0 == 0) {
+                        const u64 target = !by_p ? ~0ull : stage == 0 ? share_of(share, (double)o.total) : target_p;
+                        Part best{0.0, m, -1.0f, 0.0f, top, 0x7fffffff};
+                        u64 before = o.before;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            if (i0 + i < kept && before < target && o.e[i] >= (d.min_p > 0.0f ? d.min_p : 0.0f)) {
+                                const int v = (int)(unsigned int)s.list[i0 + i];
+                                const float score = __fdividef(o.e[i], q[v]);
+                                if (better(score, v, best.score, best.index)) best.score = score, best.index = v, best.z = o.z[i];
+                            }
+                            before += o.w[i];
+                        }
+                        best = block_part(best, s);
+                        if (threadIdx.x == 0) {
+                            const bool drawn = best.index != 0x7fffffff;  // (noise of NaN alone: the most likely token)
+                            token[row] = drawn ? best.index : top;
+                            if (logprob) logprob[row] = ((drawn ? best.z : m) - m) - log_sum(all);
+                        }
+                        return;
+                    }
+                    // the cut to every CTA
+                    Cut cut{0, 0x7fffffff, o.total, true};
+                    if (stage == 0) {
+                        cut.key = (unsigned int)(s.list[kept - 1] >> 32);
+                    } else {
+                        u64 before = o.before;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            if (i0 + i < kept && before < target_p && before + o.w[i] >= target_p) s.place = i0 + i;
+                            before += o.w[i];
+                        }
+                        __syncthreads();
+                        cut.key = (unsigned int)(s.list[s.place] >> 32), cut.index = (int)(unsigned int)s.list[s.place] + 1;
+                    }
+                    if ((int)threadIdx.x < C) cl.map_shared_rank(&s, threadIdx.x)->cut[stage] = cut;
+                }
+                if (right) {
+                    cl.sync();
+                    (stage == 0 ? cut_k : cut_p) = s.cut[stage];
+                    done = true;
+                }
+            }
+            if (!done) {
+                const Cut cut = descend(zs, slice, first, m, s, cl, stage == 1, stage == 0 ? (u64)k : target_p);
+                (stage == 0 ? cut_k : cut_p) = cut;
+            }
         }
     }
     const unsigned int key = cut_k.key < cut_p.key ? cut_k.key : cut_p.key;
-    Exchange best{0.0, -1.0f, 0.0f, 0x7fffffff};
-    const float* q = noise + row * noise_ld;
-    for (int j = threadIdx.x; j < slice; j += THREADS) {
-        const float z = zs[j];
-        if (z == -INFINITY) continue;
-        const float e = expf(z - m);
-        best.sum += (double)e;  // (a sure token's log-probability is all in the small terms)
-        if (greedy) continue;
-        const unsigned int k = down_key(z);
-        const int v = first + j;
-        if (k <= key && e >= min_p && !(k == cut_p.key && v >= cut_p.index)) {
-            const float score = e / q[v];
-            if (better(score, v, best.value, best.index)) best.value = score, best.index = v, best.z = z;
-        }
-    }
-    best = cluster_best(best, s, 1, cl);
-    if (rank == 0 && threadIdx.x == 0) {
-        const bool drawn = !greedy && best.index != 0x7fffffff;  // (noise of NaN alone: the most likely token)
-        token[row] = drawn ? best.index : top;
-        if (logprob) logprob[row] = (float)((double)((drawn ? best.z : m) - m) - log(best.sum));
-    }
+    const float least = d.min_p > 0.0f ? d.min_p : 0.0f;
+    finish<VEC>(zs, slice, first, m, top, d, q, logprob != nullptr, s, cl, token + row, logprob ? logprob + row : nullptr,
+                [&](float z, int v, float e) {
+                    const unsigned int kk = down_key(z);
+                    return kk <= key && e >= least && !(kk == cut_p.key && v >= cut_p.index);
+                });
 }
 
 }  // namespace rwkv7
@@ -487,23 +929,28 @@ extern "C" int rwkv7_sample_tokens(const void* logits, int64_t ld, const rwkv7_l
     while (C < MAX_CLUSTER && V > 4096 * C) C *= 2;
     const int64_t places = (int64_t)V + vec - 1;  // a row may begin up to vec - 1 places into its first vector
     const int64_t slice = ((places + C - 1) / C + vec - 1) / vec * vec;
-    const int64_t smem = (sizeof(Shared) + 15) / 16 * 16 + slice * 4;
+    const bool filters = noise && (draw->top_k || (draw->top_k_value > 0 && draw->top_k_value < V) || draw->top_p || draw->top_p_value < 1.0f);
+    const bool ruled = rules->tokens || rules->bias || rules->allowed;
+    const int64_t smem = (filters ? FILTER_SHARED : PICK_SHARED) + slice * 4;
     RWKV7_REQUIRE(smem <= 227 * 1024, RWKV7_ERR_UNSUPPORTED, "sample_tokens: a vocabulary of %d tokens does not fit the shared memory of a cluster", V);
     RWKV7_REQUIRE((int64_t)B * C < (1ll << 31), RWKV7_ERR_UNSUPPORTED, "sample_tokens: too many rows (%d)", B);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     RWKV7_DISPATCH_DTYPE(dtype, T, {
-        auto kernel = sample_kernel<T>;
+        auto kernel = filters ? (ruled ? filter_kernel<T, true> : filter_kernel<T, false>) : ruled ? pick_kernel<T, true> : pick_kernel<T, false>;
         const cudaError_t a = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         RWKV7_REQUIRE(a == cudaSuccess, RWKV7_ERR_CUDA, "sample_tokens: %s", cudaGetErrorString(a));
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)(B * C));
         cfg.blockDim = dim3(THREADS);
         cfg.dynamicSmemBytes = (size_t)smem;
-        cfg.stream = static_cast<cudaStream_t>(stream);
-        cudaLaunchAttribute attr[1];
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = C, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        cfg.numAttrs = programmatic_launch_ok(st) ? 2 : 1;
         cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), ld, *rules, *draw, noise, noise_ld, token, logprob, V, (int)slice);
     });
     return check_launch("sample_kernel");
