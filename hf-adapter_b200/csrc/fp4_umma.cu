@@ -2,42 +2,48 @@
 //
 //   y[m, n] = epilogue( gx[m] * gw[n] * sum_k q_x[m, k] s_x[m, k / block] q_w[n, k] s_w[n, k / block] )
 //
-// The weight is operand A (128 output channels a tile: the lanes of the accumulator), the tokens are operand B (the
-// columns), so one kernel serves one token and thousands.  A stage of the ring holds 256 elements of K: codes by TMA in
-// the 128-byte swizzle that the MMA reads, scale tiles by plain bulk copies (they lie in memory as tensor memory wants them).
-// Warp 0 = producer, warp 1 = MMA issuer (copies a stage's scales to tensor memory, then issues its MMAs of 64 k; both
-// run in issue order), warps 2-5 = epilogue.  All waits are bounded (umma.cuh).
+// A stage of either kernel's ring holds 256 elements of K (128 bytes a row) of both operands, by TMA in the 128-byte swizzle that the
+// MMA reads, and their scale tiles, which lie in memory as tensor memory wants them.  The MMA thread copies a stage's
+// scales to tensor memory and issues its MMAs of 64 k behind them; both run in issue order, and a stage's columns of
+// scales are written again only when its MMAs are known to be done (the stage's `empty` barrier).
+//
+// Few tokens (stream kernel): the weight is operand A (128 output channels: the lanes of the accumulator), the tokens are
+// operand B (the columns), so that one token costs a tile of 128 x 16 and not one of 128 x 128; K is split over the CTAs of a cluster
+// where the channels alone do not fill the GPU.  Many tokens (pair kernel): tokens are operand A, CTA pairs on tiles of
+// 256 x 256 or 256 x 128, persistent.  All waits are bounded (umma.cuh).
+#include <cooperative_groups.h>
+
 #include "fp4.cuh"
 #include "umma.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace rwkv7 {
 namespace f4 {
-constexpr int BM = 128, BKB = 128, THREADS = 192;  // channels a tile, bytes (256 elements) of K a stage
-constexpr int A_BYTES = BM * BKB;
+constexpr int KS = 256, KSB = 128;  // elements and bytes of K a stage
 constexpr int tiles_per_stage(int format) { return format == fp4::MX ? 2 : 4; }  // scale tiles of 128 rows
-constexpr int sf_rows(int bn) { return (bn + 127) / 128; }
 constexpr int sf_bytes(int format) { return tiles_per_stage(format) * fp4::SCALE_TILE_BYTES; }
-constexpr int stage_bytes(int format, int bn) { return A_BYTES + bn * BKB + (1 + sf_rows(bn)) * sf_bytes(format); }
-constexpr int stages(int bn) { return bn == 256 ? 4 : 6; }
 constexpr int BAR_BYTES = 1024;
-constexpr int smem_bytes(int format, int bn) { return stages(bn) * stage_bytes(format, bn) + BAR_BYTES + bn * 4 + 1024; }
-// tensor memory: the accumulator, then per stage the scales of A (4 columns a tile) and of B
-constexpr int sf_cols(int format, int bn) { return tiles_per_stage(format) * 4 * (1 + sf_rows(bn)); }
-constexpr int tmem_cols(int format, int bn) {
-    int need = bn + stages(bn) * sf_cols(format, bn), c = 32;
+constexpr int pow2_cols(int need) {
+    int c = 32;
     while (c < need) c *= 2;
     return c;
 }
 }  // namespace f4
 
 struct Fp4Args {
-    const uint8_t *ws, *xs;        // scale tiles of the weight and the tokens
-    const float *wg, *xg;          // row factors (nvfp4; NULL = 1)
+    const float *wg, *xg;  // row factors (nvfp4; NULL = 1)
     const void *bias, *residual;
     void* y;
     int M, N, K;
     int relu2;
+    int vec;     // rows of y and the residual allow 16-byte accesses
+    int splits;  // stream kernel: CTAs of a cluster that share a K range
+    int tiles_m, tiles_n;
     unsigned int* error;
+};
+struct Fp4Maps {
+    CUtensorMap w, x, ws, xs, y;  // codes, scale tiles, and (pair kernel) the output
 };
 
 // Instruction descriptor of the block-scaled 4-bit kinds: E2M1 operands (1), scale type (0 = E4M3, 1 = E8M0), and which
@@ -45,148 +51,207 @@ struct Fp4Args {
 __host__ __device__ constexpr uint32_t fp4_idesc(int M, int N, int e8m0, uint32_t sf_id) {
     return (sf_id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)e8m0 << 23) | ((uint32_t)(M >> 7) << 27) | (sf_id << 29);
 }
-template <int FORMAT>
+template <int FORMAT, int GROUP>
 __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    if constexpr (FORMAT == fp4::MX)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+#define RWKV7_FP4_MMA(KIND)                                                                              \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                        \
+                 "tcgen05.mma.cta_group::%7." KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}"               \
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "n"(GROUP) : "memory")
+    if constexpr (FORMAT == fp4::MX) RWKV7_FP4_MMA("kind::mxf4.block_scale.scale_vec::2X");
+    else RWKV7_FP4_MMA("kind::mxf4nvf4.block_scale.scale_vec::4X");
+#undef RWKV7_FP4_MMA
 }
-// One scale tile (32 rows of 16 bytes, 8-row groups 128 bytes apart) to four columns, repeated in the four lane quarters
-__device__ __forceinline__ void copy_scale_tile(uint32_t taddr, uint32_t smem_addr) {
-    uint64_t d = (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+// Descriptor of a scale tile (32 rows of 16 bytes, 8-row groups 128 bytes apart, no swizzle), and its copy to four columns,
+// repeated in the four lane quarters
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
-__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint64_t* bar, uint32_t bytes) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+template <int GROUP> __device__ __forceinline__ void copy_scale_tile(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::%2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc), "n"(GROUP) : "memory");
+}
+__device__ __forceinline__ bool elect_lane() {  // (the compiler knows that one thread runs what this guards)
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}" : "=r"(pred));
+    return pred != 0;
 }
 
+// The scale copies and MMAs of one stage, `steps` of 64 k of it (4, fewer at a ragged end).  BR: scale tiles of operand B beside one another.
+template <int FORMAT, int GROUP, int M, int N, int BR>
+__device__ __forceinline__ void issue_stage(uint32_t d, uint64_t da, uint64_t db, uint32_t sfa, uint64_t sf_a, uint64_t sf_b, int steps, bool first) {
+    constexpr int TPS = f4::tiles_per_stage(FORMAT);
+    constexpr uint32_t id0 = fp4_idesc(M, N, FORMAT == fp4::MX, 0), id2 = fp4_idesc(M, N, 1, 2);
+    const uint32_t sfb = sfa + TPS * 4;
+#pragma unroll
+    for (int t = 0; t < TPS; ++t) {
+        copy_scale_tile<GROUP>(sfa + 4 * t, sf_a + (uint64_t)(t * (fp4::SCALE_TILE_BYTES >> 4)));
+#pragma unroll
+        for (int r = 0; r < BR; ++r)
+            copy_scale_tile<GROUP>(sfb + 4 * (t * BR + r), sf_b + (uint64_t)((r * TPS + t) * (fp4::SCALE_TILE_BYTES >> 4)));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int t = FORMAT == fp4::MX ? j >> 1 : j;
+        if (j < steps)
+            umma_fp4<FORMAT, GROUP>(d, da + (uint64_t)(j * 2), db + (uint64_t)(j * 2), FORMAT == fp4::MX && (j & 1) ? id2 : id0, sfa + 4 * t,
+                                    sfb + 4 * BR * t, first && j == 0 ? 0u : 1u);
+    }
+}
+
+// ---------------------------------------------------------------- few tokens
+namespace fs {
+constexpr int BM = 128, THREADS = 192, A_BYTES = BM * f4::KSB, MAX_SPLITS = 8;
+constexpr int stage_bytes(int format, int bn) { return A_BYTES + bn * f4::KSB + 2 * f4::sf_bytes(format); }
+constexpr int stages(int bn) { return bn <= 32 ? 8 : bn == 64 ? 7 : 5; }
+constexpr int smem_bytes(int format, int bn) { return stages(bn) * stage_bytes(format, bn) + f4::BAR_BYTES + 1024; }
+constexpr int sf_cols(int format) { return f4::tiles_per_stage(format) * 8; }
+constexpr int tmem_cols(int format, int bn) { return f4::pow2_cols(bn + stages(bn) * sf_cols(format)); }
+}  // namespace fs
+
+// grid (channel tiles, token tiles, splits); warp 0 = producer, warp 1 = MMA, warps 2..5 read the accumulator, all write the result
 template <int FORMAT, typename T, int BN>
-__global__ void __launch_bounds__(f4::THREADS, 1)
-fp4_umma_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Fp4Args p) {
-    using namespace f4;
-    constexpr int STAGES = stages(BN), STAGE_BYTES = stage_bytes(FORMAT, BN), TPS = tiles_per_stage(FORMAT), SFR = sf_rows(BN);
-    constexpr int SFB_BYTES = sf_bytes(FORMAT), TMEM_COLS = tmem_cols(FORMAT, BN), SF_COLS = sf_cols(FORMAT, BN);
-    static_assert(BN + STAGES * SF_COLS <= TMEM_COLS && TMEM_COLS <= 512, "tensor memory");
+__global__ void __launch_bounds__(fs::THREADS, 1) fp4_stream_kernel(const __grid_constant__ Fp4Maps maps, const Fp4Args p) {
+    using namespace fs;
+    constexpr int STAGES = stages(BN), SF = f4::sf_bytes(FORMAT), TMEM_COLS = tmem_cols(FORMAT, BN), STAGE_BYTES = stage_bytes(FORMAT, BN);
+    static_assert(BN + STAGES * sf_cols(FORMAT) <= TMEM_COLS && TMEM_COLS <= 512, "tensor memory");
+    static_assert(BN * BM * 4 <= STAGES * STAGE_BYTES, "the exchange takes the ring's place");
     extern __shared__ unsigned char smem_unaligned[];
     unsigned char* sm = smem_unaligned + ((1024u - (smem_u32(smem_unaligned) & 1023u)) & 1023u);
-    // [A of all stages][B of all stages][scales of all stages][barriers][row factors of the tokens]
+    // [A of all stages][B of all stages][scales of all stages][barriers]; behind the last MMA [split][token][channel] in fp32
     unsigned char* sm_b = sm + STAGES * A_BYTES;
-    unsigned char* sm_s = sm_b + STAGES * BN * BKB;
+    unsigned char* sm_s = sm_b + STAGES * BN * f4::KSB;
+    float* Q = reinterpret_cast<float*>(sm);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + STAGES * STAGE_BYTES);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* s_xg = reinterpret_cast<float*>(sm + STAGES * STAGE_BYTES + BAR_BYTES);
     const AbortCtx actx{abort_flag, p.error};
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = tid & 31;
     const int n0 = blockIdx.x * BM, m0 = blockIdx.y * BN;
-    const int nk = (p.K + 2 * BKB - 1) / (2 * BKB);
-    const int ktiles = fp4::k_tiles(p.K, FORMAT);
+    const int all = (p.K + f4::KS - 1) / f4::KS, split = blockIdx.z;
+    const int kb0 = split * all / p.splits, nk = (split + 1) * all / p.splits - kb0;  // at least one stage each
+    const bool clustered = p.splits > 1;
 
     if (tid == 0) {
-        tma_prefetch_desc(&tm_w);
-        tma_prefetch_desc(&tm_x);
         for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
         mbar_init(acc_full, 1);
         *abort_flag = 0;
         mbar_fence_init();
+        tma_prefetch_desc(&maps.w), tma_prefetch_desc(&maps.ws), tma_prefetch_desc(&maps.x), tma_prefetch_desc(&maps.xs);
+        // the weight does not depend on the kernel before this one: what the ring holds is requested under it
+        for (int i = 0; i < STAGES && i < nk; ++i) {
+            mbar_expect_tx(&full[i], STAGE_BYTES);
+            tma_load_2d(sm + i * A_BYTES, &maps.w, &full[i], (kb0 + i) * f4::KSB, n0);
+            tma_load_2d(sm_s + i * 2 * SF, &maps.ws, &full[i], (kb0 + i) * (SF / 8), blockIdx.x);
+        }
     }
     if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
-    for (int i = tid; i < BN; i += THREADS) s_xg[i] = p.xg && m0 + i < p.M ? p.xg[m0 + i] : 1.0f;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0) {
-        if (lane == 0) {
-            const int x_tiles = (p.M + 127) / 128, rt = m0 / 128;
-            const int sfb_rows = x_tiles - rt < SFR ? x_tiles - rt : SFR;  // scale row-tiles that exist
-            for (int kb = 0; kb < nk; ++kb) {
-                const int s = kb % STAGES;
-                if (kb >= STAGES && !mbar_wait(&empty[s], ((kb / STAGES) - 1) & 1, actx, kErrWaitEmpty)) break;
-                const int kt = kb * TPS, live = ktiles - kt < TPS ? ktiles - kt : TPS;
-                const uint32_t sf = live * fp4::SCALE_TILE_BYTES;
-                mbar_expect_tx(&full[s], A_BYTES + BN * BKB + sf * (1 + sfb_rows));
-                tma_load_2d(sm + s * A_BYTES, &tm_w, &full[s], kb * BKB, n0);
-                tma_load_2d(sm_b + s * BN * BKB, &tm_x, &full[s], kb * BKB, m0);
-                unsigned char* sf_dst = sm_s + s * (1 + SFR) * SFB_BYTES;
-                bulk_load(sf_dst, p.ws + ((size_t)blockIdx.x * ktiles + kt) * fp4::SCALE_TILE_BYTES, &full[s], sf);
-                for (int r = 0; r < sfb_rows; ++r)
-                    bulk_load(sf_dst + (1 + r) * SFB_BYTES, p.xs + ((size_t)(rt + r) * ktiles + kt) * fp4::SCALE_TILE_BYTES, &full[s], sf);
+        if (elect_lane()) {
+            grid_dependency_wait();
+            grid_launch_dependents();
+            for (int i = 0; i < nk; ++i) {
+                const int s = i % STAGES, kb = kb0 + i;
+                if (i >= STAGES) {
+                    if (!mbar_wait(&empty[s], ((i / STAGES) - 1) & 1, actx, kErrWaitEmpty)) break;
+                    mbar_expect_tx(&full[s], STAGE_BYTES);
+                    tma_load_2d(sm + s * A_BYTES, &maps.w, &full[s], kb * f4::KSB, n0);
+                    tma_load_2d(sm_s + s * 2 * SF, &maps.ws, &full[s], kb * (SF / 8), blockIdx.x);
+                }
+                tma_load_2d(sm_b + s * BN * f4::KSB, &maps.x, &full[s], kb * f4::KSB, m0);
+                tma_load_2d(sm_s + s * 2 * SF + SF, &maps.xs, &full[s], kb * (SF / 8), m0 / 128);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_lane()) {
             bool ok = true;
-            for (int kb = 0; kb < nk; ++kb) {
-                const int s = kb % STAGES;
-                if (!mbar_wait_hot(&full[s], (kb / STAGES) & 1, actx, kErrWaitFull)) {
+            for (int i = 0; i < nk; ++i) {
+                const int s = i % STAGES;
+                if (!mbar_wait_hot(&full[s], (i / STAGES) & 1, actx, kErrWaitFull)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const int steps = (p.K - kb * 256 + 63) / 64 < 4 ? (p.K - kb * 256 + 63) / 64 : 4;  // of 64 elements
-                const uint32_t sfa = tmem + BN + s * SF_COLS, sfb = sfa + TPS * 4;
-                const uint32_t sf_src = smem_u32(sm_s + s * (1 + SFR) * SFB_BYTES);
-                for (int t = 0; t < TPS; ++t) {
-                    if (t * 4 / TPS >= steps) break;
-                    copy_scale_tile(sfa + 4 * t, sf_src + t * fp4::SCALE_TILE_BYTES);
-#pragma unroll
-                    for (int r = 0; r < SFR; ++r)
-                        copy_scale_tile(sfb + 4 * (t * SFR + r), sf_src + (1 + r) * SFB_BYTES + t * fp4::SCALE_TILE_BYTES);
-                }
-                const uint64_t da = make_sw128_kmajor_desc(smem_u32(sm + s * A_BYTES));
-                const uint64_t db = make_sw128_kmajor_desc(smem_u32(sm_b + s * BN * BKB));
-                for (int j = 0; j < steps; ++j) {
-                    const int t = FORMAT == fp4::MX ? j >> 1 : j;
-                    const uint32_t id = FORMAT == fp4::MX && (j & 1) ? fp4_idesc(BM, BN, 1, 2) : fp4_idesc(BM, BN, FORMAT == fp4::MX, 0);
-                    umma_fp4<FORMAT>(tmem, da + (uint64_t)(j * 2), db + (uint64_t)(j * 2), id, sfa + 4 * t, sfb + 4 * SFR * t,
-                                     kb > 0 || j > 0);
-                }
+                const uint64_t sf = scale_desc(smem_u32(sm_s + s * 2 * SF));
+                issue_stage<FORMAT, 1, BM, BN, 1>(tmem, make_sw128_kmajor_desc(smem_u32(sm + s * A_BYTES)),
+                                                  make_sw128_kmajor_desc(smem_u32(sm_b + s * BN * f4::KSB)), tmem + BN + s * sf_cols(FORMAT), sf,
+                                                  sf + (uint64_t)(SF >> 4), (p.K - (kb0 + i) * f4::KS + 63) / 64, i == 0);
                 tc_commit(&empty[s]);
             }
             if (ok) tc_commit(acc_full);
         }
-    } else {
-        const int q = warp & 3, n = n0 + q * 32 + lane;
-        bool ok = true;
-        if (lane == 0) ok = mbar_wait(acc_full, 0, actx, kErrWaitDFull);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (ok) {
-            tc_fence_after();
-            const float gw = p.wg && n < p.N ? p.wg[n] : 1.0f;
-            const float b = p.bias && n < p.N ? to_f<T>(static_cast<const T*>(p.bias)[n]) : 0.0f;
+    }
+    __syncwarp();
+
+    // every MMA of this CTA is done: the ring is free, here and (behind the cluster barrier) in the other CTAs
+    bool ok = true;
+    if (lane == 0) ok = mbar_wait(acc_full, 0, actx, kErrWaitDFull);
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    cg::cluster_group cl = cg::this_cluster();
+    if (clustered) cl.sync();
+    else __syncthreads();
+    const int per = BN / p.splits, rows = min(BN, p.M - m0);  // tokens a CTA finishes, tokens of the tile
+    if (warp >= 2 && ok) {
+        tc_fence_after();
+        const int q = warp & 3, ch = q * 32 + lane;
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 16) {
-                if (m0 + c >= p.M) break;
-                uint32_t v[16];
-                tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
-                tc_wait_ld();
-                if (n < p.N) {
+        for (int c = 0; c < rows; c += 8) {
+            uint32_t v[8];
+            tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+            tc_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int m = m0 + c + i;
-                        if (m < p.M) {
-                            float y = __uint_as_float(v[i]) * (gw * s_xg[c + i]) + b;
-                            if (p.relu2) y = y > 0.0f ? y * y : y != y ? y : 0.0f;
-                            if (p.residual) y += to_f<T>(static_cast<const T*>(p.residual)[(size_t)m * p.N + n]);
-                            static_cast<T*>(p.y)[(size_t)m * p.N + n] = from_f<T>(y);
-                        }
-                    }
-                }
+            for (int i = 0; i < 8; ++i) {
+                const int to = (c + i) / per;
+                float* dst = Q + ((size_t)(clustered ? split * per : 0) + (c + i - to * per)) * BM + ch;
+                if (c + i < rows) *(clustered ? cl.map_shared_rank(dst, to) : dst + (size_t)to * per * BM) = __uint_as_float(v[i]);
             }
-            tc_fence_before();
+        }
+        tc_fence_before();
+    }
+    if (clustered) cl.sync();
+    else __syncthreads();
+    if (*abort_flag == 0) {
+        grid_dependency_wait();  // (returns at once; the row factors and the residual are read, the result is written behind it)
+        const int t0 = clustered ? split * per : 0, t1 = min(rows, clustered ? t0 + per : rows);
+        for (int idx = tid; idx < (t1 - t0) * (BM / 4); idx += THREADS) {
+            const int t = idx / (BM / 4), ch = idx % (BM / 4) * 4, m = m0 + t0 + t, n = n0 + ch;
+            if (n >= p.N) continue;
+            const float* src = Q + t * BM + ch;
+            float4 a = *reinterpret_cast<const float4*>(src);
+            for (int r = 1; clustered && r < p.splits; ++r) {
+                const float4 b = *reinterpret_cast<const float4*>(src + (size_t)r * per * BM);
+                a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
+            }
+            const float gx = p.xg ? p.xg[m] : 1.0f;
+            float y[4] = {a.x, a.y, a.z, a.w};
+            const size_t o = (size_t)m * p.N + n;
+            const T* bias = static_cast<const T*>(p.bias);
+            const T* res = p.residual ? static_cast<const T*>(p.residual) + o : nullptr;
+            T* out = static_cast<T*>(p.y) + o;
+            float r4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const bool whole = p.vec && n + 4 <= p.N;
+            if (res) {
+                if (whole) load4<T>(res, r4);
+                else
+                    for (int e = 0; e < 4 && n + e < p.N; ++e) r4[e] = to_f<T>(res[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int ne = n + e < p.N ? n + e : p.N - 1;
+                y[e] *= gx * (p.wg ? p.wg[ne] : 1.0f);
+                if (bias) y[e] += to_f<T>(bias[ne]);
+                if (p.relu2) y[e] = y[e] > 0.0f ? y[e] * y[e] : y[e] != y[e] ? y[e] : 0.0f;
+                y[e] += r4[e];
+            }
+            if (whole) store4<T>(out, y);
+            else
+                for (int e = 0; e < 4 && n + e < p.N; ++e) out[e] = from_f<T>(y[e]);
         }
     }
     __syncthreads();
@@ -196,26 +261,287 @@ fp4_umma_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
     }
 }
 
-template <int FORMAT, typename T, int BN>
-static int launch_fp4(const void* w, const void* xq, const Fp4Args& a, cudaStream_t st) {
-    CUtensorMap tm_w, tm_x;
-    if (int e = make_tmap_2d(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.N, a.K / 2, f4::BM, f4::BKB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
-    if (int e = make_tmap_2d(&tm_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, a.M, a.K / 2, BN, f4::BKB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
-    auto kernel = fp4_umma_kernel<FORMAT, T, BN>;
-    constexpr int smem = f4::smem_bytes(FORMAT, BN);
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    RWKV7_REQUIRE(e == cudaSuccess, RWKV7_ERR_CUDA, "fp4_linear: %s", cudaGetErrorString(e));
-    kernel<<<dim3((a.N + f4::BM - 1) / f4::BM, (a.M + BN - 1) / BN), f4::THREADS, smem, st>>>(tm_w, tm_x, a);
-    return check_launch("fp4_umma_kernel");
+// ---------------------------------------------------------------- many tokens
+// Roles and barriers as in gemm_umma_pair_kernel (gemm_umma.cu): both producers' loads complete on the leader's full[s]; the
+// leader's commits arrive on empty[s] / acc_full[a] in both CTAs; the epilogue warps of both arrive on the leader's acc_empty[a].
+// Each CTA stages its own 128 token rows, half of the channels, the scales of its own rows and those of all channels
+// (each CTA's tensor memory needs them).  Eight epilogue warps, two a lane quarter, each with half of the columns.
+namespace fp {
+constexpr int BM = 128, PAIR_M = 256, EW = 8, THREADS = 64 + 32 * EW, STAGES = 5, A_BYTES = BM * f4::KSB, GROUP_M = 16;
+constexpr int b_bytes(int bn) { return bn / 2 * f4::KSB; }
+constexpr int sfb_rows(int bn) { return bn / 128; }
+constexpr int stage_bytes(int format, int bn) { return A_BYTES + b_bytes(bn) + (1 + sfb_rows(bn)) * f4::sf_bytes(format); }
+constexpr int accs(int bn) { return bn == 256 ? 1 : 2; }
+constexpr int sf_cols(int format, int bn) { return f4::tiles_per_stage(format) * 4 * (1 + sfb_rows(bn)); }
+constexpr int STG_WARP_BYTES = 4096;  // 32 rows x 128 bytes
+constexpr int vec_bytes(int bn) { return 2 * bn * 4; }  // channel factors and bias of a tile
+constexpr int smem_bytes(int format, int bn) { return STAGES * stage_bytes(format, bn) + EW * STG_WARP_BYTES + f4::BAR_BYTES + vec_bytes(bn) + 1024; }
+constexpr int TMEM_COLS = 512;
+}  // namespace fp
+
+__device__ __forceinline__ void fp4_tile(int tile, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int per_band = fp::GROUP_M * tiles_n, band = tile / per_band, within = tile - band * per_band;
+    const int rows = min(fp::GROUP_M, tiles_m - band * fp::GROUP_M);
+    tn = within / rows;
+    tm = band * fp::GROUP_M + (within - tn * rows);
 }
 
-// (a tile narrower than 128 tokens is used for a first tile alone: the scales of its tokens begin in the first column of their tile)
+template <int FORMAT, typename T, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp::THREADS, 1) fp4_pair_kernel(const __grid_constant__ Fp4Maps maps, const Fp4Args p) {
+    using namespace fp;
+    constexpr int SF = f4::sf_bytes(FORMAT), SFR = sfb_rows(BN), STAGE_BYTES = stage_bytes(FORMAT, BN), ACCS = accs(BN), B_BYTES = b_bytes(BN);
+    static_assert(ACCS * BN + STAGES * sf_cols(FORMAT, BN) <= TMEM_COLS, "tensor memory");
+    static_assert(smem_bytes(FORMAT, BN) <= 227 * 1024, "shared memory");
+    extern __shared__ unsigned char smem_unaligned[];
+    unsigned char* sm = smem_unaligned + ((1024u - (smem_u32(smem_unaligned) & 1023u)) & 1023u);
+    // [A of all stages][B of all stages][output staging][scales of all stages][barriers][channel factors, bias]
+    unsigned char* sm_b = sm + STAGES * A_BYTES;
+    unsigned char* sm_o = sm_b + STAGES * B_BYTES;
+    unsigned char* sm_s = sm_o + EW * STG_WARP_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm_s + STAGES * (1 + SFR) * SF);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;
+    uint64_t* acc_empty = acc_full + ACCS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + ACCS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* s_wg = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(full) + f4::BAR_BYTES);
+    float* s_bias = s_wg + BN;
+    const AbortCtx actx{abort_flag, p.error};
+
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = tid & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int nk = (p.K + f4::KS - 1) / f4::KS, ntiles = p.tiles_m * p.tiles_n;
+
+    if (tid == 0) {
+        tma_prefetch_desc(&maps.w), tma_prefetch_desc(&maps.ws), tma_prefetch_desc(&maps.x), tma_prefetch_desc(&maps.xs);
+        for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        for (int a = 0; a < ACCS; ++a) mbar_init(&acc_full[a], 1), mbar_init(&acc_empty[a], 2 * EW);
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    // the peer's barriers must exist before anything of this CTA signals them
+    cluster_arrive_release();
+    cluster_wait();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    if (warp == 0) {
+        if (elect_lane()) {
+            int it = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < ntiles; tile += npairs) {
+                int tm, tn;
+                fp4_tile(tile, p.tiles_m, p.tiles_n, tm, tn);
+                const int row_a = tm * PAIR_M + (int)rank * BM, row_b = tn * BN + (int)rank * (BN / 2);
+                for (int kb = 0; kb < nk; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    if (it >= STAGES && !mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, actx, kErrWaitEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    if (leader) mbar_expect_tx(&full[s], 2 * STAGE_BYTES);
+                    const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+                    tma_load_2d_pair(sm + s * A_BYTES, &maps.x, bar, kb * f4::KSB, row_a);
+                    tma_load_2d_pair(sm_b + s * B_BYTES, &maps.w, bar, kb * f4::KSB, row_b);
+                    unsigned char* sf = sm_s + s * (1 + SFR) * SF;
+                    tma_load_2d_pair(sf, &maps.xs, bar, kb * (SF / 8), row_a / 128);
+                    tma_load_2d_pair(sf + SF, &maps.ws, bar, kb * (SF / 8), tn * SFR);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (leader && elect_lane()) {
+            int it = 0, li = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < ntiles; tile += npairs, ++li) {
+                const int as = li % ACCS;
+                if (li >= ACCS && !mbar_wait_hot(&acc_empty[as], ((li / ACCS) - 1) & 1, actx, kErrWaitDFull)) break;
+                tc_fence_after();
+                for (int kb = 0; kb < nk; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait_hot(&full[s], (it / STAGES) & 1, actx, kErrWaitFull)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t sf = scale_desc(smem_u32(sm_s + s * (1 + SFR) * SF));
+                    issue_stage<FORMAT, 2, PAIR_M, BN, SFR>(tmem + as * BN, make_sw128_kmajor_desc(smem_u32(sm + s * A_BYTES)),
+                                                            make_sw128_kmajor_desc(smem_u32(sm_b + s * B_BYTES)),
+                                                            tmem + ACCS * BN + s * sf_cols(FORMAT, BN), sf, sf + (uint64_t)(SF >> 4),
+                                                            (p.K - kb * f4::KS + 63) / 64, kb == 0);
+                    tc_commit_pair(&empty[s]);
+                }
+                if (ok) tc_commit_pair(&acc_full[as]);
+            }
+        }
+    } else {
+        const int q = warp & 3, half = (warp - 2) >> 2, et = tid - 64;  // (this thread among the epilogue's)
+        constexpr int GROUPS = BN / 128;  // of 64 columns a warp
+        unsigned char* stg = sm_o + (warp - 2) * STG_WARP_BYTES;
+        const T* bias = static_cast<const T*>(p.bias);
+        const T* res = static_cast<const T*>(p.residual);
+        int li = 0;
+        for (int tile = pair; tile < ntiles; tile += npairs, ++li) {
+            const int as = li % ACCS;
+            int tm, tn;
+            fp4_tile(tile, p.tiles_m, p.tiles_n, tm, tn);
+            // the tile's channel factors and bias (the warps meet on a barrier of their own: the last tile's are no longer read)
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            for (int i = et; i < BN; i += 32 * EW) {
+                const int n = tn * BN + i < p.N ? tn * BN + i : p.N - 1;
+                s_wg[i] = p.wg ? p.wg[n] : 1.0f;
+                s_bias[i] = bias ? to_f<T>(bias[n]) : 0.0f;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const int row0 = tm * PAIR_M + (int)rank * BM + q * 32, row = row0 + lane;
+            const float gx = p.xg && row < p.M ? p.xg[row] : 1.0f;
+            bool ok = true;
+            if (lane == 0) ok = mbar_wait(&acc_full[as], (li / ACCS) & 1, actx, kErrWaitDFull);
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) continue;  // (not out of the loop: the warps still meet at its barriers)
+            tc_fence_after();
+#pragma unroll 1
+            for (int g = 0; g < GROUPS; ++g) {
+                const int c0 = (half * GROUPS + g) * 64, col0 = tn * BN + c0;
+                uint32_t v[64];
+                tmem_ld64(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(as * BN + c0), v);
+                tc_wait_ld();
+                if (g == GROUPS - 1) {  // the accumulator has been read: the next tile may overwrite it
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (leader) mbar_arrive(&acc_empty[as]);
+                        else mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[as]), 0));
+                    }
+                }
+                if (row0 >= p.M || col0 >= p.N) continue;
+                const size_t o = (size_t)row * p.N + col0;
+                const bool bulk = sizeof(T) == 2 && p.vec;
+                if (bulk && lane == 0) tma_store_wait_read<0>();  // the last group's copy has left the staging tile
+                __syncwarp();
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    float f[8], r[8];
+                    const float4 w0 = *reinterpret_cast<const float4*>(s_wg + c0 + 8 * u), w1 = *reinterpret_cast<const float4*>(s_wg + c0 + 8 * u + 4);
+                    const float4 b0 = *reinterpret_cast<const float4*>(s_bias + c0 + 8 * u), b1 = *reinterpret_cast<const float4*>(s_bias + c0 + 8 * u + 4);
+                    const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w}, b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+                    const bool here = row < p.M && col0 + 8 * u + 8 <= p.N;
+                    if (res) {
+                        if (here && p.vec) load8<T>(res + o + 8 * u, r);
+                        else
+                            for (int e = 0; e < 8; ++e) r[e] = row < p.M && col0 + 8 * u + e < p.N ? to_f<T>(res[o + 8 * u + e]) : 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        f[e] = fmaf(__uint_as_float(v[8 * u + e]), gx * w[e], b[e]);
+                        if (p.relu2) f[e] = f[e] > 0.0f ? f[e] * f[e] : f[e] != f[e] ? f[e] : 0.0f;
+                        if (res) f[e] += r[e];
+                    }
+                    if (bulk) store8<T>(reinterpret_cast<T*>(stg + lane * 128 + ((u ^ (lane & 7)) << 4)), f);
+                    else if (here && p.vec) store8<T>(static_cast<T*>(p.y) + o + 8 * u, f);
+                    else if (row < p.M)
+                        for (int e = 0; e < 8 && col0 + 8 * u + e < p.N; ++e) static_cast<T*>(p.y)[o + 8 * u + e] = from_f<T>(f[e]);
+                }
+                if (bulk) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&maps.y, stg, col0, row0);
+                        tma_store_commit();
+                    }
+                }
+            }
+        }
+        if (lane == 0) tma_store_wait_all();
+    }
+    // neither CTA may free its tensor memory or leave while the other can still touch its memory
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive_release();
+    cluster_wait();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, TMEM_COLS);
+    }
+}
+
+// ---------------------------------------------------------------- host
+// scale tiles as a matrix of 8-byte words, a row-tile a row; boxes of `box_rows` row tiles x one stage
+static int make_tmap_scales(CUtensorMap* map, const void* base, int rows, int K, int format, int box_rows) {
+    return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_INT64, 8, base, (uint64_t)(rows + 127) / 128, (uint64_t)fp4::k_tiles(K, format) * 64,
+                        (uint32_t)box_rows, (uint32_t)f4::sf_bytes(format) / 8, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <int FORMAT, typename T, int BN>
+static int launch_stream(const void* w, const void* ws, const void* xq, const void* xs, Fp4Args a, cudaStream_t st) {
+    Fp4Maps m{};
+    if (int e = make_tmap_2d(&m.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.N, a.K / 2, fs::BM, f4::KSB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+    if (int e = make_tmap_2d(&m.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, a.M, a.K / 2, BN, f4::KSB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+    if (int e = make_tmap_scales(&m.ws, ws, a.N, a.K, FORMAT, 1)) return e;
+    if (int e = make_tmap_scales(&m.xs, xs, a.M, a.K, FORMAT, 1)) return e;
+    auto kernel = fp4_stream_kernel<FORMAT, T, BN>;
+    constexpr int smem = fs::smem_bytes(FORMAT, BN);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    RWKV7_REQUIRE(e == cudaSuccess, RWKV7_ERR_CUDA, "fp4_linear: %s", cudaGetErrorString(e));
+    const int tn = (a.N + fs::BM - 1) / fs::BM, tm = (a.M + BN - 1) / BN, stages = (a.K + f4::KS - 1) / f4::KS;
+    a.splits = 1;
+    while (a.splits < fs::MAX_SPLITS && 2 * a.splits <= stages && (int64_t)tn * tm * 2 * a.splits <= kSMs) a.splits *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(tn, tm, a.splits);
+    cfg.blockDim = dim3(fs::THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = a.splits;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = programmatic_launch_ok(st) ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, m, a);
+    return check_launch("fp4_stream_kernel");
+}
+
+template <int FORMAT, typename T, int BN>
+static int launch_pair(const void* w, const void* ws, const void* xq, const void* xs, Fp4Args a, cudaStream_t st) {
+    Fp4Maps m{};
+    if (int e = make_tmap_2d(&m.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.N, a.K / 2, BN / 2, f4::KSB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+    if (int e = make_tmap_2d(&m.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, a.M, a.K / 2, fp::BM, f4::KSB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+    if (int e = make_tmap_scales(&m.ws, ws, a.N, a.K, FORMAT, fp::sfb_rows(BN))) return e;
+    if (int e = make_tmap_scales(&m.xs, xs, a.M, a.K, FORMAT, 1)) return e;
+    if (sizeof(T) == 2 && a.vec) {
+        const CUtensorMapDataType dt = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;  // (bits are copied)
+        if (int e = make_tmap_2d(&m.y, dt, (int)sizeof(T), a.y, a.M, a.N, 32, 64, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+    }
+    auto kernel = fp4_pair_kernel<FORMAT, T, BN>;
+    constexpr int smem = fp::smem_bytes(FORMAT, BN);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    RWKV7_REQUIRE(e == cudaSuccess, RWKV7_ERR_CUDA, "fp4_linear: %s", cudaGetErrorString(e));
+    a.tiles_m = (a.M + fp::PAIR_M - 1) / fp::PAIR_M, a.tiles_n = (a.N + BN - 1) / BN;
+    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n;
+    const int pairs = (int)(tiles < kSMs / 2 ? tiles : kSMs / 2);
+    const cudaError_t l = launch_programmatic(kernel, dim3(2 * pairs), dim3(fp::THREADS), smem, st, m, a);
+    RWKV7_REQUIRE(l == cudaSuccess, RWKV7_ERR_CUDA, "fp4_linear: %s", cudaGetErrorString(l));
+    return check_launch("fp4_pair_kernel");
+}
+
 template <int FORMAT, typename T>
-static int dispatch_fp4(const void* w, const void* xq, const Fp4Args& a, cudaStream_t st) {
-    if (a.M <= 16) return launch_fp4<FORMAT, T, 16>(w, xq, a, st);
-    if (a.M <= 64) return launch_fp4<FORMAT, T, 64>(w, xq, a, st);
-    if (a.M <= 512) return launch_fp4<FORMAT, T, 128>(w, xq, a, st);
-    return launch_fp4<FORMAT, T, 256>(w, xq, a, st);
+static int dispatch_fp4(const void* w, const void* ws, const void* xq, const void* xs, const Fp4Args& a, cudaStream_t st) {
+    if (a.M <= 16) return launch_stream<FORMAT, T, 16>(w, ws, xq, xs, a, st);
+    if (a.M <= 32) return launch_stream<FORMAT, T, 32>(w, ws, xq, xs, a, st);
+    if (a.M <= 64) return launch_stream<FORMAT, T, 64>(w, ws, xq, xs, a, st);
+    if (a.M <= 128) return launch_stream<FORMAT, T, 128>(w, ws, xq, xs, a, st);
+    const int64_t fit = kSMs / 2, tm = (a.M + fp::PAIR_M - 1) / fp::PAIR_M;
+    const auto waves = [&](int bn) { return (tm * ((a.N + bn - 1) / bn) + fit - 1) / fit; };
+    if (waves(128) * 400 < waves(256) * 600) return launch_pair<FORMAT, T, 128>(w, ws, xq, xs, a, st);
+    return launch_pair<FORMAT, T, 256>(w, ws, xq, xs, a, st);
 }
 
 // Where the quantised tokens lie in the workspace: codes, scale tiles, row factors
@@ -260,14 +586,15 @@ extern "C" int rwkv7_fp4_linear(const void* x, int64_t ldx, const void* w_packed
     float* xg = reinterpret_cast<float*>(base + ws.row_scale);
     if (int e = launch_fp4_quant(x, ldx, base, base + ws.scales, xg, M, K, format, dtype, st)) return e;
     Fp4Args a{};
-    a.ws = static_cast<const uint8_t*>(w_scales), a.xs = base + ws.scales;
     a.wg = w_row_scale, a.xg = format == fp4::NV ? xg : nullptr;
     a.bias = bias, a.residual = residual, a.y = y;
     a.M = M, a.N = N, a.K = K, a.relu2 = epilogue == RWKV7_EPI_RELU2;
+    a.vec = N % 8 == 0 && aligned(y, 16) && (!residual || aligned(residual, 16));
     a.error = kernel_error_word();
     RWKV7_REQUIRE(a.error != nullptr, RWKV7_ERR_CUDA, "fp4_linear: cannot resolve the device error word");
     RWKV7_DISPATCH_DTYPE(dtype, T, {
-        return format == fp4::MX ? dispatch_fp4<fp4::MX, T>(w_packed, base, a, st) : dispatch_fp4<fp4::NV, T>(w_packed, base, a, st);
+        return format == fp4::MX ? dispatch_fp4<fp4::MX, T>(w_packed, w_scales, base, base + ws.scales, a, st)
+                                 : dispatch_fp4<fp4::NV, T>(w_packed, w_scales, base, base + ws.scales, a, st);
     });
     return RWKV7_OK;
 }
