@@ -99,32 +99,38 @@ __device__ __forceinline__ void issue_stage(uint32_t d, uint64_t da, uint64_t db
 
 // ---------------------------------------------------------------- few tokens
 namespace fs {
-constexpr int BM = 128, THREADS = 192, A_BYTES = BM * f4::KSB, MAX_SPLITS = 8;
+constexpr int BM = 128, EW = 8, THREADS = 64 + 32 * EW, A_BYTES = BM * f4::KSB, MAX_SPLITS = 8;
 constexpr int stage_bytes(int format, int bn) { return A_BYTES + bn * f4::KSB + 2 * f4::sf_bytes(format); }
-constexpr int stages(int bn) { return bn <= 32 ? 8 : bn == 64 ? 7 : 5; }
-constexpr int smem_bytes(int format, int bn) { return stages(bn) * stage_bytes(format, bn) + f4::BAR_BYTES + 1024; }
+constexpr int stages(int bn) { return bn <= 32 ? 8 : bn == 64 ? 6 : 4; }
+constexpr int q_bytes(int bn) { return bn * BM * 4; }  // partial sums of a tile
+constexpr int smem_bytes(int format, int bn) { return stages(bn) * stage_bytes(format, bn) + q_bytes(bn) + f4::BAR_BYTES + bn * 4 + 1024; }
 constexpr int sf_cols(int format) { return f4::tiles_per_stage(format) * 8; }
 constexpr int tmem_cols(int format, int bn) { return f4::pow2_cols(bn + stages(bn) * sf_cols(format)); }
 }  // namespace fs
 
-// grid (channel tiles, token tiles, splits); warp 0 = producer, warp 1 = MMA, warps 2..5 read the accumulator, all write the result
+// grid (channel tiles, token tiles, splits); warp 0 = producer, warp 1 = MMA, warps 2..9 = epilogue (two a lane quarter, eight
+// tokens each in turn).  A lane is a channel: what a warp stores or reads for one token is 32 neighbouring channels, whole sectors.
+// The kernel before this one in the stream is the quantiser of the tokens: only their codes, scales and row factors wait for
+// it.  It has itself waited for everything earlier before it let this kernel start, so the weight, bias and residual are there.
+// (B200, nvfp4: 1 x 4096 -> 16384 streams 37.8 MB of weight in FIXME)
 template <int FORMAT, typename T, int BN>
 __global__ void __launch_bounds__(fs::THREADS, 1) fp4_stream_kernel(const __grid_constant__ Fp4Maps maps, const Fp4Args p) {
     using namespace fs;
     constexpr int STAGES = stages(BN), SF = f4::sf_bytes(FORMAT), TMEM_COLS = tmem_cols(FORMAT, BN), STAGE_BYTES = stage_bytes(FORMAT, BN);
     static_assert(BN + STAGES * sf_cols(FORMAT) <= TMEM_COLS && TMEM_COLS <= 512, "tensor memory");
-    static_assert(BN * BM * 4 <= STAGES * STAGE_BYTES, "the exchange takes the ring's place");
+    static_assert(smem_bytes(FORMAT, BN) <= 227 * 1024, "shared memory");
     extern __shared__ unsigned char smem_unaligned[];
     unsigned char* sm = smem_unaligned + ((1024u - (smem_u32(smem_unaligned) & 1023u)) & 1023u);
-    // [A of all stages][B of all stages][scales of all stages][barriers]; behind the last MMA [split][token][channel] in fp32
+    // [A of all stages][B of all stages][scales of all stages][partial sums: split, token, channel][barriers][row factors]
     unsigned char* sm_b = sm + STAGES * A_BYTES;
     unsigned char* sm_s = sm_b + STAGES * BN * f4::KSB;
-    float* Q = reinterpret_cast<float*>(sm);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + STAGES * STAGE_BYTES);
+    float* Q = reinterpret_cast<float*>(sm + STAGES * STAGE_BYTES);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + STAGES * STAGE_BYTES + q_bytes(BN));
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* s_xg = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(full) + f4::BAR_BYTES);
     const AbortCtx actx{abort_flag, p.error};
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = tid & 31;
@@ -138,19 +144,33 @@ __global__ void __launch_bounds__(fs::THREADS, 1) fp4_stream_kernel(const __grid
         mbar_init(acc_full, 1);
         *abort_flag = 0;
         mbar_fence_init();
-        tma_prefetch_desc(&maps.w), tma_prefetch_desc(&maps.ws), tma_prefetch_desc(&maps.x), tma_prefetch_desc(&maps.xs);
         // the weight does not depend on the kernel before this one: what the ring holds is requested under it
         for (int i = 0; i < STAGES && i < nk; ++i) {
             mbar_expect_tx(&full[i], STAGE_BYTES);
             tma_load_2d(sm + i * A_BYTES, &maps.w, &full[i], (kb0 + i) * f4::KSB, n0);
             tma_load_2d(sm_s + i * 2 * SF, &maps.ws, &full[i], (kb0 + i) * (SF / 8), blockIdx.x);
         }
+        tma_prefetch_desc(&maps.x), tma_prefetch_desc(&maps.xs);
     }
     if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    cg::cluster_group cl = cg::this_cluster();
+    if (clustered) cluster_arrive_relaxed();  // this CTA runs: the others may write into its partial sums
+
+    // this thread's channel in the epilogue, its factor and bias
+    const int q = warp & 3, half = (warp - 2) >> 2, ch = q * 32 + lane, n = n0 + ch;
+    const int rows = min(BN, p.M - m0);
+    float gw = 1.0f, bias = 0.0f;
+    const T* res = p.residual ? static_cast<const T*>(p.residual) + (size_t)m0 * p.N + n : nullptr;
+    T* out = static_cast<T*>(p.y) + (size_t)m0 * p.N + n;
+    const auto result = [&](float sum, int t, float r) {
+        float y = fmaf(sum, gw * s_xg[t], bias);
+        if (p.relu2) y = y > 0.0f ? y * y : y != y ? y : 0.0f;
+        out[(size_t)t * p.N] = from_f<T>(y + r);
+    };
 
     if (warp == 0) {
         if (elect_lane()) {
@@ -186,72 +206,63 @@ __global__ void __launch_bounds__(fs::THREADS, 1) fp4_stream_kernel(const __grid
             }
             if (ok) tc_commit(acc_full);
         }
+    } else {
+        if (n < p.N) {
+            if (p.wg) gw = p.wg[n];
+            if (p.bias) bias = to_f<T>(static_cast<const T*>(p.bias)[n]);
+        }
+        grid_dependency_wait();
+        for (int t = tid - 64; t < rows; t += 32 * EW) s_xg[t] = p.xg ? p.xg[m0 + t] : 1.0f;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        bool ok = true;
+        if (lane == 0) ok = mbar_wait(acc_full, 0, actx, kErrWaitDFull);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (clustered) cluster_wait();
+        if (ok) {
+            tc_fence_after();
+            const int per = BN / p.splits, lg_per = 31 - __clz(per);  // tokens that a CTA finishes
+#pragma unroll 1
+            for (int c = 8 * half; c < rows; c += 16) {
+                float r[8];
+                if (res && !clustered) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) r[i] = c + i < rows && n < p.N ? to_f<T>(res[(size_t)(c + i) * p.N]) : 0.0f;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) r[i] = 0.0f;
+                }
+                uint32_t v[8];
+                tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+                tc_wait_ld();
+                if (!clustered) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (c + i < rows && n < p.N) result(__uint_as_float(v[i]), c + i, r[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int to = (c + i) >> lg_per;
+                        if (c + i < rows) *cl.map_shared_rank(Q + ((split << lg_per) + (c + i) - (to << lg_per)) * BM + ch, to) = __uint_as_float(v[i]);
+                    }
+                }
+            }
+            tc_fence_before();
+        }
     }
     __syncwarp();
-
-    // every MMA of this CTA is done: the ring is free, here and (behind the cluster barrier) in the other CTAs
-    bool ok = true;
-    if (lane == 0) ok = mbar_wait(acc_full, 0, actx, kErrWaitDFull);
-    ok = __shfl_sync(0xffffffffu, ok, 0);
-    cg::cluster_group cl = cg::this_cluster();
-    if (clustered) cl.sync();
-    else __syncthreads();
-    const int per = BN / p.splits, rows = min(BN, p.M - m0);  // tokens a CTA finishes, tokens of the tile
-    if (warp >= 2 && ok) {
-        tc_fence_after();
-        const int q = warp & 3, ch = q * 32 + lane;
-#pragma unroll 1
-        for (int c = 0; c < rows; c += 8) {
-            uint32_t v[8];
-            tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + c, v);
-            tc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int to = (c + i) / per;
-                float* dst = Q + ((size_t)(clustered ? split * per : 0) + (c + i - to * per)) * BM + ch;
-                if (c + i < rows) *(clustered ? cl.map_shared_rank(dst, to) : dst + (size_t)to * per * BM) = __uint_as_float(v[i]);
+    if (clustered) {
+        if (warp < 2) cluster_wait();
+        cl.sync();
+        if (warp >= 2 && n < p.N && *abort_flag == 0) {
+            // the partial sums in the order of K
+            const int per = BN / p.splits, t0 = split * per, t1 = min(rows, t0 + per);
+            for (int t = t0 + half; t < t1; t += 2) {
+                const float r = res ? to_f<T>(res[(size_t)t * p.N]) : 0.0f;
+                const float* src = Q + (t - t0) * BM + ch;
+                float sum = src[0];
+                for (int z = 1; z < p.splits; ++z) sum += src[z * per * BM];
+                result(sum, t, r);
             }
-        }
-        tc_fence_before();
-    }
-    if (clustered) cl.sync();
-    else __syncthreads();
-    if (*abort_flag == 0) {
-        grid_dependency_wait();  // (returns at once; the row factors and the residual are read, the result is written behind it)
-        const int t0 = clustered ? split * per : 0, t1 = min(rows, clustered ? t0 + per : rows);
-        for (int idx = tid; idx < (t1 - t0) * (BM / 4); idx += THREADS) {
-            const int t = idx / (BM / 4), ch = idx % (BM / 4) * 4, m = m0 + t0 + t, n = n0 + ch;
-            if (n >= p.N) continue;
-            const float* src = Q + t * BM + ch;
-            float4 a = *reinterpret_cast<const float4*>(src);
-            for (int r = 1; clustered && r < p.splits; ++r) {
-                const float4 b = *reinterpret_cast<const float4*>(src + (size_t)r * per * BM);
-                a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
-            }
-            const float gx = p.xg ? p.xg[m] : 1.0f;
-            float y[4] = {a.x, a.y, a.z, a.w};
-            const size_t o = (size_t)m * p.N + n;
-            const T* bias = static_cast<const T*>(p.bias);
-            const T* res = p.residual ? static_cast<const T*>(p.residual) + o : nullptr;
-            T* out = static_cast<T*>(p.y) + o;
-            float r4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const bool whole = p.vec && n + 4 <= p.N;
-            if (res) {
-                if (whole) load4<T>(res, r4);
-                else
-                    for (int e = 0; e < 4 && n + e < p.N; ++e) r4[e] = to_f<T>(res[e]);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int ne = n + e < p.N ? n + e : p.N - 1;
-                y[e] *= gx * (p.wg ? p.wg[ne] : 1.0f);
-                if (bias) y[e] += to_f<T>(bias[ne]);
-                if (p.relu2) y[e] = y[e] > 0.0f ? y[e] * y[e] : y[e] != y[e] ? y[e] : 0.0f;
-                y[e] += r4[e];
-            }
-            if (whole) store4<T>(out, y);
-            else
-                for (int e = 0; e < 4 && n + e < p.N; ++e) out[e] = from_f<T>(y[e]);
         }
     }
     __syncthreads();
@@ -407,20 +418,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp::THREADS, 1) fp4_
             ok = __shfl_sync(0xffffffffu, ok, 0);
             if (!ok) continue;  // (not out of the loop: the warps still meet at its barriers)
             tc_fence_after();
-#pragma unroll 1
+            // all of this warp's columns at once, then the accumulator goes back: with one accumulator the MMAs wait for this alone
+            uint32_t v[GROUPS][64];
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) tmem_ld64(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(as * BN + (half * GROUPS + g) * 64), v[g]);
+            tc_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (leader) mbar_arrive(&acc_empty[as]);
+                else mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[as]), 0));
+            }
+#pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 const int c0 = (half * GROUPS + g) * 64, col0 = tn * BN + c0;
-                uint32_t v[64];
-                tmem_ld64(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(as * BN + c0), v);
-                tc_wait_ld();
-                if (g == GROUPS - 1) {  // the accumulator has been read: the next tile may overwrite it
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (leader) mbar_arrive(&acc_empty[as]);
-                        else mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[as]), 0));
-                    }
-                }
                 if (row0 >= p.M || col0 >= p.N) continue;
                 const size_t o = (size_t)row * p.N + col0;
                 const bool bulk = sizeof(T) == 2 && p.vec;
@@ -440,7 +451,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp::THREADS, 1) fp4_
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        f[e] = fmaf(__uint_as_float(v[8 * u + e]), gx * w[e], b[e]);
+                        f[e] = fmaf(__uint_as_float(v[g][8 * u + e]), gx * w[e], b[e]);
                         if (p.relu2) f[e] = f[e] > 0.0f ? f[e] * f[e] : f[e] != f[e] ? f[e] : 0.0f;
                         if (res) f[e] += r[e];
                     }
