@@ -297,6 +297,80 @@ __device__ __forceinline__ void fp4_tile(int tile, int tiles_m, int tiles_n, int
     tm = band * fp::GROUP_M + (within - tn * rows);
 }
 
+// 64 columns of a warp's 32 rows (a lane is a row): factors and bias, then MODE 0 nothing, 1 relu^2, 2 + residual.  16-bit
+// results go through the warp's staging tile (16-byte pieces xored by the row: the layout of a 128-byte-swizzled tensor map) and
+// leave as one bulk copy, or, where rows of y are not 16-byte aligned, as coalesced single values.
+template <int FORMAT, typename T, int MODE>
+__device__ __forceinline__ void fp4_columns(const Fp4Args& p, const CUtensorMap& tm_y, const uint32_t (&v)[64], const float* wg, const float* bias, float gx,
+                                            int row0, int col0, int lane, unsigned char* stg) {
+    const int row = row0 + lane, live = row < p.M ? p.N - col0 : 0;  // columns of this row that exist
+    const size_t o = (size_t)row * p.N + col0;
+    const T* res = static_cast<const T*>(p.residual) + o;
+    if (sizeof(T) == 2) {
+        if (p.vec && lane == 0) tma_store_wait_read<0>();  // the last group's copy has left the staging tile
+        __syncwarp();
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        float f[8], r[8];
+        if constexpr (MODE == 2) {
+            if (p.vec) {
+                if (8 * u < live) load8<T>(res + 8 * u, r);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[e] = 8 * u + e < live ? to_f<T>(res[8 * u + e]) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(bias + 8 * u + h);
+            f[h] = b.x, f[h + 1] = b.y, f[h + 2] = b.z, f[h + 3] = b.w;
+            if constexpr (FORMAT == fp4::NV) {
+                const float4 w = *reinterpret_cast<const float4*>(wg + 8 * u + h);
+                f[h] = fmaf(__uint_as_float(v[8 * u + h]), gx * w.x, f[h]), f[h + 1] = fmaf(__uint_as_float(v[8 * u + h + 1]), gx * w.y, f[h + 1]);
+                f[h + 2] = fmaf(__uint_as_float(v[8 * u + h + 2]), gx * w.z, f[h + 2]), f[h + 3] = fmaf(__uint_as_float(v[8 * u + h + 3]), gx * w.w, f[h + 3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[h + e] += __uint_as_float(v[8 * u + h + e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (MODE == 1) f[e] = f[e] > 0.0f ? f[e] * f[e] : f[e] != f[e] ? f[e] : 0.0f;
+            if constexpr (MODE == 2) f[e] += r[e];
+        }
+        if constexpr (sizeof(T) == 2) {
+            store8<T>(reinterpret_cast<T*>(stg + lane * 128 + ((u ^ (lane & 7)) << 4)), f);
+        } else {
+            T* y = static_cast<T*>(p.y) + o + 8 * u;
+            if (p.vec) {
+                if (8 * u < live) store8<T>(y, f);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (8 * u + e < live) y[e] = from_f<T>(f[e]);
+            }
+        }
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (p.vec) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(&tm_y, stg, col0, row0);
+                tma_store_commit();
+            }
+        } else {
+            __syncwarp();
+            const int cols = p.N - col0 < 64 ? p.N - col0 : 64, rows = p.M - row0 < 32 ? p.M - row0 : 32;
+            for (int r = 0; r < rows; ++r)
+                for (int c = lane; c < cols; c += 32)
+                    static_cast<T*>(p.y)[(size_t)(row0 + r) * p.N + col0 + c] = *reinterpret_cast<const T*>(stg + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+            __syncwarp();
+        }
+    }
+}
+
 template <int FORMAT, typename T, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp::THREADS, 1) fp4_pair_kernel(const __grid_constant__ Fp4Maps maps, const Fp4Args p) {
     using namespace fp;
@@ -397,7 +471,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp::THREADS, 1) fp4_
         constexpr int GROUPS = BN / 128;  // of 64 columns a warp
         unsigned char* stg = sm_o + (warp - 2) * STG_WARP_BYTES;
         const T* bias = static_cast<const T*>(p.bias);
-        const T* res = static_cast<const T*>(p.residual);
         int li = 0;
         for (int tile = pair; tile < ntiles; tile += npairs, ++li) {
             const int as = li % ACCS;
@@ -429,45 +502,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp::THREADS, 1) fp4_
                 if (leader) mbar_arrive(&acc_empty[as]);
                 else mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[as]), 0));
             }
+            if (row0 >= p.M) continue;
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 const int c0 = (half * GROUPS + g) * 64, col0 = tn * BN + c0;
-                if (row0 >= p.M || col0 >= p.N) continue;
-                const size_t o = (size_t)row * p.N + col0;
-                const bool bulk = sizeof(T) == 2 && p.vec;
-                if (bulk && lane == 0) tma_store_wait_read<0>();  // the last group's copy has left the staging tile
-                __syncwarp();
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    float f[8], r[8];
-                    const float4 w0 = *reinterpret_cast<const float4*>(s_wg + c0 + 8 * u), w1 = *reinterpret_cast<const float4*>(s_wg + c0 + 8 * u + 4);
-                    const float4 b0 = *reinterpret_cast<const float4*>(s_bias + c0 + 8 * u), b1 = *reinterpret_cast<const float4*>(s_bias + c0 + 8 * u + 4);
-                    const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w}, b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
-                    const bool here = row < p.M && col0 + 8 * u + 8 <= p.N;
-                    if (res) {
-                        if (here && p.vec) load8<T>(res + o + 8 * u, r);
-                        else
-                            for (int e = 0; e < 8; ++e) r[e] = row < p.M && col0 + 8 * u + e < p.N ? to_f<T>(res[o + 8 * u + e]) : 0.0f;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        f[e] = fmaf(__uint_as_float(v[g][8 * u + e]), gx * w[e], b[e]);
-                        if (p.relu2) f[e] = f[e] > 0.0f ? f[e] * f[e] : f[e] != f[e] ? f[e] : 0.0f;
-                        if (res) f[e] += r[e];
-                    }
-                    if (bulk) store8<T>(reinterpret_cast<T*>(stg + lane * 128 + ((u ^ (lane & 7)) << 4)), f);
-                    else if (here && p.vec) store8<T>(static_cast<T*>(p.y) + o + 8 * u, f);
-                    else if (row < p.M)
-                        for (int e = 0; e < 8 && col0 + 8 * u + e < p.N; ++e) static_cast<T*>(p.y)[o + 8 * u + e] = from_f<T>(f[e]);
-                }
-                if (bulk) {
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&maps.y, stg, col0, row0);
-                        tma_store_commit();
-                    }
-                }
+                if (col0 >= p.N) continue;
+                if (p.relu2) fp4_columns<FORMAT, T, 1>(p, maps.y, v[g], s_wg + c0, s_bias + c0, gx, row0, col0, lane, stg);
+                else if (p.residual) fp4_columns<FORMAT, T, 2>(p, maps.y, v[g], s_wg + c0, s_bias + c0, gx, row0, col0, lane, stg);
+                else fp4_columns<FORMAT, T, 0>(p, maps.y, v[g], s_wg + c0, s_bias + c0, gx, row0, col0, lane, stg);
             }
         }
         if (lane == 0) tma_store_wait_all();
