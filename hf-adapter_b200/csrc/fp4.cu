@@ -45,131 +45,202 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
     return byte == 255 ? __int_as_float(0x7fffffff) : byte ? __int_as_float(byte << 23) : __int_as_float(1 << 22);
 }
 
-// the largest finite magnitude of 16 elements, and whether all are finite
-__device__ __forceinline__ float finite_amax(const float (&v)[16], bool& finite) {
-    float m = 0.0f;
-    finite = true;
+// 16 elements as they lie in memory
+template <typename T> struct Piece {
+    uint4 w[sizeof(T)];  // (sizeof(T) = 16 elements x sizeof(T) / 16)
+};
+template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T* p) {
+    Piece<T> o;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float a = fabsf(v[i]);
-        const bool ok = a < INFINITY;  // false for NaN too
-        finite &= ok;
-        m = fmaxf(m, ok ? a : 0.0f);
+    for (int i = 0; i < (int)sizeof(T); ++i) o.w[i] = reinterpret_cast<const uint4*>(p)[i];
+    return o;
+}
+template <typename T> __device__ __forceinline__ void widen(const Piece<T>& p, float (&v)[16]) {
+    const T* e = reinterpret_cast<const T*>(p.w);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = to_f<T>(e[i]);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+template <typename T> struct Two;
+template <> struct Two<__half> { typedef __half2 type; };
+template <> struct Two<__nv_bfloat16> { typedef __nv_bfloat162 type; };
+// the largest magnitude of a piece, infinite or NaN if an element is
+template <typename T> __device__ __forceinline__ float piece_amax(const Piece<T>& p) {
+    if constexpr (sizeof(T) == 4) {
+        const float* e = reinterpret_cast<const float*>(p.w);
+        float m = fabsf(e[0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) m = max_nan(m, fabsf(e[i]));
+        return m;
+    } else if constexpr (sizeof(T) == 2) {
+        typedef typename Two<T>::type T2;
+        const T2* e = reinterpret_cast<const T2*>(p.w);
+        T2 m = __habs2(e[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(e[i]));
+        return max_nan(to_f<T>(m.x), to_f<T>(m.y));
+    }
+}
+// the same over the finite elements alone
+template <typename T> __device__ __forceinline__ float finite_amax(const Piece<T>& p) {
+    float m = piece_amax(p);
+    if (!(m < INFINITY)) {
+        float v[16];
+        widen(p, v);
+        m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (fabsf(v[i]) < INFINITY) m = fmaxf(m, fabsf(v[i]));
     }
     return m;
 }
 
-template <typename T> __device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
+// Codes and the block's scale byte of one piece; g's exponent byte, inv_g = 1 / g (nvfp4).  Whole warps.
+template <typename T, int FORMAT>
+__device__ __forceinline__ uint32_t encode_piece(const Piece<T>& piece, int ge, uint2& codes) {
+    float v[16];
+    widen(piece, v);
+    float m = piece_amax(piece);
+    uint32_t byte;
+    if constexpr (FORMAT == MX) {
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        const bool finite = m < INFINITY;
+        byte = finite ? max((__float_as_int(m) >> 23) - 2, 0) : 255;
+        const float mult = __int_as_float(finite ? (254 - byte) << 23 : 0);  // 2^(127 - byte); byte <= 252
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float o[8];
-        load8<T>(p + 8 * h, o);
+        for (int i = 0; i < 16; ++i) v[i] *= mult;
+    } else {
+        const float inv_g = __int_as_float((254 - ge) << 23);
+        byte = __nv_cvt_float_to_fp8(m * inv_g * (1.0f / 6.0f), __NV_SATFINITE, __NV_E4M3);
+        float s = e4m3_value(byte), inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+        if (!(m < INFINITY)) byte = 0x7f;
+        if (ge >= 32 && ge <= 224) {  // the powers of two in one factor (exact: nothing leaves the range)
+            inv *= inv_g, s *= __int_as_float(ge << 23);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * h + i] = o[i];
+            for (int i = 0; i < 16; ++i) v[i] *= inv_g;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float q = v[i] * inv;
+            v[i] = fmaf(fmaf(-q, s, v[i]), inv, q);
+        }
     }
+    float lo[8], hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lo[i] = v[i], hi[i] = v[8 + i];
+    codes = make_uint2(pack8(lo), pack8(hi));
+    return byte;
 }
 
-// A CTA a row, 16 elements a thread and pass.  Rows beyond R pad the last scale tile with zeros.
-template <typename T, int FORMAT>
+// `team` threads a row, P pieces of 16 elements a thread, read once and kept (P = 0: read again for the codes).  Rows beyond R
+// pad the last scale tile with zeros.  Bound by the memory: FIXME
+template <typename T, int FORMAT, int P>
 __global__ void __launch_bounds__(256) fp4_quant_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ packed,
-                                                        uint8_t* __restrict__ scales, float* __restrict__ row_scale, int R, int K) {
-    __shared__ float red[32];
-    const int64_t row = blockIdx.x;
-    const int ktiles = k_tiles(K, FORMAT), pieces = K / 16;
+                                                        uint8_t* __restrict__ scales, float* __restrict__ row_scale, int R, int K, int team) {
+    __shared__ float red[8];
+    const int at = threadIdx.x % team, lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / team) + threadIdx.x / team;
+    const int ktiles = k_tiles(K, FORMAT), pieces = row < R ? K / 16 : 0;
     const int padded = ktiles * SCALE_TILE_BLOCKS * block_of(FORMAT) / 16;  // pieces that the scale tiles cover
-    const int lane = threadIdx.x & 31;
-    if (row >= R) {
-        for (int t = threadIdx.x; t < ktiles; t += blockDim.x) *reinterpret_cast<uint32_t*>(scales + scale_word(row, t, ktiles)) = 0;
-        return;
-    }
+    grid_dependency_wait();
+    grid_launch_dependents();
     const T* xr = x + row * ldx;
-    float inv_g = 1.0f;
-    if (FORMAT == NV) {
-        float m = 0.0f;
-        for (int p = threadIdx.x; p < pieces; p += blockDim.x) {
-            float v[16];
-            bool finite;
-            load16<T>(xr + 16 * p, v);
-            m = fmaxf(m, finite_amax(v, finite));
+    Piece<T> kept[P ? P : 1];
+    if constexpr (P > 0) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int p = at + i * team;
+            kept[i] = Piece<T>{};
+            if (p < pieces) kept[i] = load_piece<T>(xr + 16 * p);
         }
-        m = block_max(m, red);
-        const int e = max(__float_as_int(m) >> 23, 1);  // biased exponent; subnormal magnitudes count as the smallest normal
-        const int ge = m > 0.0f ? max(e - 10, 1) : 127;
-        inv_g = __int_as_float((254 - ge) << 23);
-        if (threadIdx.x == 0) row_scale[row] = __int_as_float(ge << 23);
     }
-    // whole warps stay in the loop for the shuffles
-    for (int p0 = threadIdx.x - lane; p0 < padded; p0 += blockDim.x) {
-        const int p = p0 + lane;
-        const bool live = p < pieces;
-        float v[16];
-        if (live) load16<T>(xr + 16 * p, v);
-        else {
+    int ge = 127;
+    if constexpr (FORMAT == NV) {
+        float m = 0.0f;
+        if constexpr (P > 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-        }
-        bool finite;
-        float m = finite_amax(v, finite);
-        uint32_t byte;
-        float mult;
-        if (FORMAT == MX) {
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            finite = __shfl_xor_sync(0xffffffffu, (int)finite, 1) && finite;
-            byte = max((__float_as_int(m) >> 23) - 2, 0);
-            mult = __int_as_float((254 - byte) << 23);  // 2^(127 - byte); byte <= 252
-            if (!finite) byte = 255;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] *= mult;
+            for (int i = 0; i < P; ++i) m = fmaxf(m, finite_amax(kept[i]));
         } else {
-            byte = __nv_cvt_float_to_fp8(m * inv_g * (1.0f / 6.0f), __NV_SATFINITE, __NV_E4M3);
-            const float s = e4m3_value(byte);
-            const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
-            if (!finite) byte = 0x7f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float u = v[i] * inv_g, q = u * inv;
-                v[i] = fmaf(fmaf(-q, s, u), inv, q);
-            }
+            for (int p = at; p < pieces; p += team) m = fmaxf(m, finite_amax(load_piece<T>(xr + 16 * p)));
         }
-        if (live) {
-            float lo[8], hi[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) lo[i] = v[i], hi[i] = v[8 + i];
-            *reinterpret_cast<uint2*>(packed + row * (K / 2) + 8 * p) = make_uint2(pack8(lo), pack8(hi));
-        } else {
-            byte = 0;
+        m = group_max<32>(m);
+        if (team > 32) {
+            if (lane == 0) red[threadIdx.x >> 5] = m;
+            __syncthreads();
+            for (int w = threadIdx.x / team * (team / 32), n = team / 32; n > 0; ++w, --n) m = fmaxf(m, red[w]);
         }
+        const int e = max(__float_as_int(m) >> 23, 1);  // biased exponent; subnormal magnitudes count as the smallest normal
+        ge = m > 0.0f ? max(e - 10, 1) : 127;
+        if (at == 0 && row < R) row_scale[row] = __int_as_float(ge << 23);
+    }
+    const auto put = [&](const Piece<T>& piece, int p) {
+        uint2 codes;
+        uint32_t byte = encode_piece<T, FORMAT>(piece, ge, codes);
+        if (p < pieces) *reinterpret_cast<uint2*>(packed + row * (K / 2) + 8 * p) = codes;
+        else byte = 0;
         // four scales to one word: blocks lie one (nvfp4) or two (mxfp4) lanes apart
         constexpr int STEP = block_of(FORMAT) / 16;
-        uint32_t word = byte;
-#pragma unroll
-        for (int i = 1; i < 4; ++i) word |= __shfl_down_sync(0xffffffffu, byte, i * STEP) << (8 * i);
+        uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, STEP) << 8;
+        word |= __shfl_down_sync(0xffffffffu, word, 2 * STEP) << 16;
         if (lane % (4 * STEP) == 0 && p < padded) *reinterpret_cast<uint32_t*>(scales + scale_word(row, p / (4 * STEP), ktiles)) = word;
+    };
+    if constexpr (P > 0) {
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+            if (at - lane + i * team < padded) put(kept[i], at + i * team);  // (whole warps, for the shuffles)
+    } else {
+        for (int p0 = at - lane; p0 < padded; p0 += team) {
+            const int p = p0 + lane;
+            Piece<T> one{};
+            if (p < pieces) one = load_piece<T>(xr + 16 * p);
+            put(one, p);
+        }
     }
 }
 
-template <typename T, int FORMAT>
+// 16 bytes of values a thread, four of them a turn; INDEX wide enough to count them
+template <typename T, int FORMAT, typename INDEX>
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t* __restrict__ packed, const uint8_t* __restrict__ scales,
-                                                          const float* __restrict__ row_scale, T* __restrict__ out, int64_t total, int K) {
-    const int pieces = K / 16, ktiles = k_tiles(K, FORMAT);
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = i / pieces;
-        const int p = (int)(i - row * pieces);
-        const int block = FORMAT == MX ? p >> 1 : p;
-        const uint32_t byte = scales[scale_word(row, block >> 2, ktiles) + (block & 3)];
-        const float s = FORMAT == MX ? e8m0_value(byte) : e4m3_value(byte);
-        const float g = FORMAT == MX || row_scale == nullptr ? 1.0f : row_scale[row];
-        const uint2 c = *reinterpret_cast<const uint2*>(packed + i * 8);
+                                                          const float* __restrict__ row_scale, T* __restrict__ out, INDEX total, int K) {
+    constexpr int E = 16 / sizeof(T);  // elements
+    const unsigned pieces = K / E;
+    const int ktiles = k_tiles(K, FORMAT);
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const INDEX stride = (INDEX)gridDim.x * blockDim.x;
+    for (INDEX i0 = (INDEX)blockIdx.x * blockDim.x + threadIdx.x; i0 < total; i0 += 4 * stride) {
+        uint32_t code[4], byte[4];
+        float g[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t w = h ? c.y : c.x;
-            float o[8];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = unpack2((w >> (8 * j)) & 255);
-                o[2 * j] = f.x * s * g, o[2 * j + 1] = f.y * s * g;
+        for (int u = 0; u < 4; ++u) {
+            const INDEX i = i0 + u * stride;
+            if (i < total) {
+                const INDEX row = i / pieces;
+                const int block = (int)(i - row * pieces) * E / block_of(FORMAT);
+                code[u] = E == 8 ? *reinterpret_cast<const uint32_t*>(packed + (int64_t)i * (E / 2)) : *reinterpret_cast<const uint16_t*>(packed + (int64_t)i * (E / 2));
+                byte[u] = scales[scale_word((int64_t)row, block >> 2, ktiles) + (block & 3)];
+                g[u] = FORMAT == MX || row_scale == nullptr ? 1.0f : row_scale[row];
             }
-            store8<T>(out + i * 16 + 8 * h, o);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const INDEX i = i0 + u * stride;
+            if (i < total) {
+                const float s = FORMAT == MX ? e8m0_value(byte[u]) : e4m3_value(byte[u]);
+                float o[E];
+#pragma unroll
+                for (int j = 0; j < E / 2; ++j) {
+                    const float2 f = unpack2((code[u] >> (8 * j)) & 255);
+                    o[2 * j] = f.x * s * g[u], o[2 * j + 1] = f.y * s * g[u];
+                }
+                if constexpr (E == 8) store8<T>(out + (int64_t)i * E, o);
+                else store4<T>(out + (int64_t)i * E, o);
+            }
         }
     }
 }
@@ -178,9 +249,17 @@ template <typename T, int FORMAT>
 static int quant(const void* x, int64_t ldx, uint8_t* packed, uint8_t* scales, float* row_scale, int rows, int K, cudaStream_t st) {
     const int ktiles = k_tiles(K, FORMAT);
     const int pieces = ktiles * SCALE_TILE_BLOCKS * block_of(FORMAT) / 16;
-    const int threads = pieces >= 256 ? 256 : (pieces + 31) / 32 * 32;
-    const int64_t grid = ((int64_t)rows + SCALE_TILE_ROWS - 1) / SCALE_TILE_ROWS * SCALE_TILE_ROWS;
-    fp4_quant_kernel<T, FORMAT><<<(unsigned)grid, threads, 0, st>>>(static_cast<const T*>(x), ldx, packed, scales, row_scale, rows, K);
+    // Few rows: a piece a thread, for the shortest way.  Many rows: four, and several rows a CTA.  (FIXME)
+    const int per = rows >= 512 ? 4 : 1;
+    int team = 32;
+    while (team < 256 && team * per < pieces) team *= 2;
+    const int threads = rows >= 512 ? 256 : team;
+    const int64_t all = ((int64_t)rows + SCALE_TILE_ROWS - 1) / SCALE_TILE_ROWS * SCALE_TILE_ROWS, grid = all / (threads / team);
+    auto kernel = pieces <= team ? fp4_quant_kernel<T, FORMAT, 1> : pieces <= 2 * team ? fp4_quant_kernel<T, FORMAT, 2>
+                  : pieces <= 4 * team ? fp4_quant_kernel<T, FORMAT, 4> : fp4_quant_kernel<T, FORMAT, 0>;
+    const cudaError_t e = launch_programmatic(kernel, dim3((unsigned)grid), dim3(threads), 0, st, static_cast<const T*>(x), ldx, packed, scales,
+                                              row_scale, rows, K, team);
+    RWKV7_REQUIRE(e == cudaSuccess, RWKV7_ERR_CUDA, "fp4_quant: %s", cudaGetErrorString(e));
     return check_launch("fp4_quant_kernel");
 }
 
@@ -221,15 +300,24 @@ extern "C" int rwkv7_fp4_dequant(const void* packed, const void* scales, const f
     RWKV7_REQUIRE(rows > 0 && K > 0, RWKV7_ERR_INVALID, "fp4_dequant: sizes must be positive");
     RWKV7_REQUIRE(format == MX || format == NV, RWKV7_ERR_INVALID, "fp4_dequant: unknown format %d", format);
     RWKV7_REQUIRE(K % 32 == 0, RWKV7_ERR_UNSUPPORTED, "fp4_dequant: K must be a multiple of 32 (got %d)", K);
+    RWKV7_REQUIRE(dtype >= RWKV7_F16 && dtype <= RWKV7_F32, RWKV7_ERR_INVALID, "fp4_dequant: unknown dtype %d", dtype);
     RWKV7_REQUIRE(packed && scales && out, RWKV7_ERR_INVALID, "fp4_dequant: null pointer");
     RWKV7_REQUIRE(aligned(packed, 16) && aligned(scales, 16) && aligned(out, 16), RWKV7_ERR_ALIGN, "fp4_dequant: tensors must be 16-byte aligned");
-    const int64_t total = (int64_t)rows * (K / 16);
-    const unsigned grid = (unsigned)((total + 255) / 256 < 16 * kSMs ? (total + 255) / 256 : 16 * kSMs);
+    const int64_t total = (int64_t)rows * (K / (16 / (int)dtype_size(dtype))), turns = (total + 1023) / 1024;
+    const unsigned grid = (unsigned)(turns < 8 * kSMs ? turns : 8 * kSMs);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const auto *c = static_cast<const uint8_t*>(packed), *s = static_cast<const uint8_t*>(scales);
+    cudaError_t e = cudaSuccess;
     RWKV7_DISPATCH_DTYPE(dtype, T, {
-        auto kernel = format == MX ? fp4_dequant_kernel<T, MX> : fp4_dequant_kernel<T, NV>;
-        kernel<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(packed), static_cast<const uint8_t*>(scales), row_scale,
-                                     static_cast<T*>(out), total, K);
+        T* o = static_cast<T*>(out);
+        if (total < (1ll << 31)) {  // (the turns after the last one stay inside 32 bits too)
+            auto kernel = format == MX ? fp4_dequant_kernel<T, MX, uint32_t> : fp4_dequant_kernel<T, NV, uint32_t>;
+            e = launch_programmatic(kernel, dim3(grid), dim3(256), 0, st, c, s, row_scale, o, (uint32_t)total, K);
+        } else {
+            auto kernel = format == MX ? fp4_dequant_kernel<T, MX, int64_t> : fp4_dequant_kernel<T, NV, int64_t>;
+            e = launch_programmatic(kernel, dim3(grid), dim3(256), 0, st, c, s, row_scale, o, total, K);
+        }
     });
+    RWKV7_REQUIRE(e == cudaSuccess, RWKV7_ERR_CUDA, "fp4_dequant: %s", cudaGetErrorString(e));
     return check_launch("fp4_dequant_kernel");
 }
