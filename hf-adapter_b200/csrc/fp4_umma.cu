@@ -100,25 +100,31 @@ __device__ __forceinline__ void issue_stage(uint32_t d, uint64_t da, uint64_t db
 // ---------------------------------------------------------------- few tokens
 namespace fs {
 constexpr int BM = 128, EW = 8, THREADS = 64 + 32 * EW, A_BYTES = BM * f4::KSB, MAX_SPLITS = 8;
+constexpr int tokens_at_once(int bn) { return bn >= 64 ? 16 : 8; }  // of an epilogue warp
 constexpr int stage_bytes(int format, int bn) { return A_BYTES + bn * f4::KSB + 2 * f4::sf_bytes(format); }
-constexpr int stages(int bn) { return bn <= 32 ? 8 : bn == 64 ? 6 : 4; }
+// DEEP: as many stages as fit, for grids of at most a CTA an SM; else room for two CTAs an SM where the tile is narrow
+constexpr int stages(int bn, bool deep) { return bn == 16 ? (deep ? 8 : 4) : bn == 32 ? (deep ? 8 : 3) : bn == 64 ? 6 : 4; }
 constexpr int q_bytes(int bn) { return bn * BM * 4; }  // partial sums of a tile
-constexpr int smem_bytes(int format, int bn) { return stages(bn) * stage_bytes(format, bn) + q_bytes(bn) + f4::BAR_BYTES + bn * 4 + 1024; }
+constexpr int smem_bytes(int format, int bn, bool deep) {
+    return stages(bn, deep) * stage_bytes(format, bn) + q_bytes(bn) + f4::BAR_BYTES + bn * 4 + 1024;
+}
 constexpr int sf_cols(int format) { return f4::tiles_per_stage(format) * 8; }
-constexpr int tmem_cols(int format, int bn) { return f4::pow2_cols(bn + stages(bn) * sf_cols(format)); }
+constexpr int tmem_cols(int format, int bn, bool deep) { return f4::pow2_cols(bn + stages(bn, deep) * sf_cols(format)); }
 }  // namespace fs
 
-// grid (channel tiles, token tiles, splits); warp 0 = producer, warp 1 = MMA, warps 2..9 = epilogue (two a lane quarter, eight
-// tokens each in turn).  A lane is a channel: what a warp stores or reads for one token is 32 neighbouring channels, whole sectors.
+// grid (channel tiles, token tiles, splits); warp 0 = producer, warp 1 = MMA, warps 2..9 = epilogue (two a lane quarter,
+// in turn).  A lane is a channel: what a warp stores or reads for one token is 32 neighbouring channels, whole sectors.
 // The kernel before this one in the stream is the quantiser of the tokens: only their codes, scales and row factors wait for
 // it.  It has itself waited for everything earlier before it let this kernel start, so the weight, bias and residual are there.
 // (B200, nvfp4: 1 x 4096 -> 16384 streams 37.8 MB of weight in FIXME)
-template <int FORMAT, typename T, int BN>
-__global__ void __launch_bounds__(fs::THREADS, 1) fp4_stream_kernel(const __grid_constant__ Fp4Maps maps, const Fp4Args p) {
+template <int FORMAT, typename T, int BN, bool DEEP>
+__global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(const __grid_constant__ Fp4Maps maps, const Fp4Args p) {
     using namespace fs;
-    constexpr int STAGES = stages(BN), SF = f4::sf_bytes(FORMAT), TMEM_COLS = tmem_cols(FORMAT, BN), STAGE_BYTES = stage_bytes(FORMAT, BN);
+    constexpr int STAGES = stages(BN, DEEP), SF = f4::sf_bytes(FORMAT), TMEM_COLS = tmem_cols(FORMAT, BN, DEEP), STAGE_BYTES = stage_bytes(FORMAT, BN);
+    constexpr int TB = tokens_at_once(BN);
     static_assert(BN + STAGES * sf_cols(FORMAT) <= TMEM_COLS && TMEM_COLS <= 512, "tensor memory");
-    static_assert(smem_bytes(FORMAT, BN) <= 227 * 1024, "shared memory");
+    static_assert(smem_bytes(FORMAT, BN, DEEP) <= (DEEP ? 227 : 113) * 1024, "shared memory");
+    static_assert(DEEP || TMEM_COLS <= 256, "tensor memory for two");
     extern __shared__ unsigned char smem_unaligned[];
     unsigned char* sm = smem_unaligned + ((1024u - (smem_u32(smem_unaligned) & 1023u)) & 1023u);
     // [A of all stages][B of all stages][scales of all stages][partial sums: split, token, channel][barriers][row factors]
@@ -164,7 +170,8 @@ __global__ void __launch_bounds__(fs::THREADS, 1) fp4_stream_kernel(const __grid
     const int q = warp & 3, half = (warp - 2) >> 2, ch = q * 32 + lane, n = n0 + ch;
     const int rows = min(BN, p.M - m0);
     float gw = 1.0f, bias = 0.0f;
-    const T* res = p.residual ? static_cast<const T*>(p.residual) + (size_t)m0 * p.N + n : nullptr;
+    // (residual reads are clamped to tokens and channels that exist, so that they need no branch and stay in flight together)
+    const T* res = p.residual ? static_cast<const T*>(p.residual) + (size_t)m0 * p.N + min(n, p.N - 1) : nullptr;
     T* out = static_cast<T*>(p.y) + (size_t)m0 * p.N + n;
     const auto result = [&](float sum, int t, float r) {
         float y = fmaf(sum, gw * s_xg[t], bias);
@@ -222,25 +229,25 @@ __global__ void __launch_bounds__(fs::THREADS, 1) fp4_stream_kernel(const __grid
             tc_fence_after();
             const int per = BN / p.splits, lg_per = 31 - __clz(per);  // tokens that a CTA finishes
 #pragma unroll 1
-            for (int c = 8 * half; c < rows; c += 16) {
-                float r[8];
+            for (int c = TB * half; c < rows; c += 2 * TB) {
+                T r[TB];
+#pragma unroll
+                for (int i = 0; i < TB; ++i) r[i] = from_f<T>(0.0f);
                 if (res && !clustered) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) r[i] = c + i < rows && n < p.N ? to_f<T>(res[(size_t)(c + i) * p.N]) : 0.0f;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) r[i] = 0.0f;
+                    for (int i = 0; i < TB; ++i) r[i] = res[(size_t)min(c + i, rows - 1) * p.N];
                 }
-                uint32_t v[8];
-                tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+                uint32_t v[TB];
+                if constexpr (TB == 16) tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+                else tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + c, v);
                 tc_wait_ld();
                 if (!clustered) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (c + i < rows && n < p.N) result(__uint_as_float(v[i]), c + i, r[i]);
+                    for (int i = 0; i < TB; ++i)
+                        if (c + i < rows && n < p.N) result(__uint_as_float(v[i]), c + i, to_f<T>(r[i]));
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < TB; ++i) {
                         const int to = (c + i) >> lg_per;
                         if (c + i < rows) *cl.map_shared_rank(Q + ((split << lg_per) + (c + i) - (to << lg_per)) * BM + ch, to) = __uint_as_float(v[i]);
                     }
@@ -252,18 +259,34 @@ __global__ void __launch_bounds__(fs::THREADS, 1) fp4_stream_kernel(const __grid
     __syncwarp();
     if (clustered) {
         if (warp < 2) cluster_wait();
-        cl.sync();
-        if (warp >= 2 && n < p.N && *abort_flag == 0) {
-            // the partial sums in the order of K
-            const int per = BN / p.splits, t0 = split * per, t1 = min(rows, t0 + per);
-            for (int t = t0 + half; t < t1; t += 2) {
-                const float r = res ? to_f<T>(res[(size_t)t * p.N]) : 0.0f;
-                const float* src = Q + (t - t0) * BM + ch;
-                float sum = src[0];
-                for (int z = 1; z < p.splits; ++z) sum += src[z * per * BM];
-                result(sum, t, r);
+        // the partial sums in the order of K, four tokens at a time, the first ones' residual requested under the barrier
+        const int per = BN / p.splits, t0 = split * per, t1 = min(rows, t0 + per);
+        const int tb = warp >= 2 && n < p.N ? t0 + half : t1;  // (the producer and MMA warps, and channels beyond N, have no token)
+        T r[4];
+        const auto residuals = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = from_f<T>(0.0f);
+            if (res && t < t1) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = res[(size_t)min(t + 2 * i, t1 - 1) * p.N];
             }
-        }
+        };
+        residuals(tb);
+        cl.sync();
+        if (*abort_flag == 0)
+            for (int t = tb; t < t1; t += 8) {
+                if (t > tb) residuals(t);
+                float sum[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float* src = Q + (t + 2 * i < t1 ? t + 2 * i - t0 : 0) * BM + ch;
+                    sum[i] = src[0];
+                    for (int z = 1; z < p.splits; ++z) sum[i] += src[z * per * BM];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t + 2 * i < t1) result(sum[i], t + 2 * i, to_f<T>(r[i]));
+            }
     }
     __syncthreads();
     if (warp == 1) {
@@ -532,20 +555,28 @@ static int make_tmap_scales(CUtensorMap* map, const void* base, int rows, int K,
                         (uint32_t)box_rows, (uint32_t)f4::sf_bytes(format) / 8, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <int FORMAT, typename T, int BN>
+// CTAs that share the K range of a tile: as many as fit beside one another and keep two stages each.  us a call, 1 / 2 / 4 / 8, 16
+// tokens: 768 -> 768 (three stages) 5.0 / 5.7 / - / -; 2560 -> 2560 7.0 / 6.6 / 6.1 / 9.9 (not all resident); 4096 -> 4096 8.7 / 7.6 / 6.7 /
+// 13.9; 16384 -> 4096 21.8 / 14.8 / 12.0 / 21.0; 4096 -> 16384 9.1 / 14.0 / 20.6 / 38.2
+static int stream_splits(int64_t tiles, int stages) {
+    int splits = 1;
+    while (splits < fs::MAX_SPLITS && 4 * splits <= stages && tiles * 2 * splits <= kSMs) splits *= 2;
+    return splits;
+}
+
+template <int FORMAT, typename T, int BN, bool DEEP>
 static int launch_stream(const void* w, const void* ws, const void* xq, const void* xs, Fp4Args a, cudaStream_t st) {
     Fp4Maps m{};
     if (int e = make_tmap_2d(&m.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.N, a.K / 2, fs::BM, f4::KSB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
     if (int e = make_tmap_2d(&m.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, a.M, a.K / 2, BN, f4::KSB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
     if (int e = make_tmap_scales(&m.ws, ws, a.N, a.K, FORMAT, 1)) return e;
     if (int e = make_tmap_scales(&m.xs, xs, a.M, a.K, FORMAT, 1)) return e;
-    auto kernel = fp4_stream_kernel<FORMAT, T, BN>;
-    constexpr int smem = fs::smem_bytes(FORMAT, BN);
+    auto kernel = fp4_stream_kernel<FORMAT, T, BN, DEEP>;
+    constexpr int smem = fs::smem_bytes(FORMAT, BN, DEEP);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     RWKV7_REQUIRE(e == cudaSuccess, RWKV7_ERR_CUDA, "fp4_linear: %s", cudaGetErrorString(e));
-    const int tn = (a.N + fs::BM - 1) / fs::BM, tm = (a.M + BN - 1) / BN, stages = (a.K + f4::KS - 1) / f4::KS;
-    a.splits = 1;
-    while (a.splits < fs::MAX_SPLITS && 2 * a.splits <= stages && (int64_t)tn * tm * 2 * a.splits <= kSMs) a.splits *= 2;
+    const int tn = (a.N + fs::BM - 1) / fs::BM, tm = (a.M + BN - 1) / BN;
+    a.splits = DEEP ? stream_splits((int64_t)tn * tm, (a.K + f4::KS - 1) / f4::KS) : 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(tn, tm, a.splits);
     cfg.blockDim = dim3(fs::THREADS);
@@ -587,13 +618,21 @@ static int launch_pair(const void* w, const void* ws, const void* xq, const void
 
 template <int FORMAT, typename T>
 static int dispatch_fp4(const void* w, const void* ws, const void* xq, const void* xs, const Fp4Args& a, cudaStream_t st) {
-    if (a.M <= 16) return launch_stream<FORMAT, T, 16>(w, ws, xq, xs, a, st);
-    if (a.M <= 32) return launch_stream<FORMAT, T, 32>(w, ws, xq, xs, a, st);
-    if (a.M <= 64) return launch_stream<FORMAT, T, 64>(w, ws, xq, xs, a, st);
-    if (a.M <= 128) return launch_stream<FORMAT, T, 128>(w, ws, xq, xs, a, st);
+    const int tiles = (a.N + fs::BM - 1) / fs::BM, stages = (a.K + f4::KS - 1) / f4::KS;
+    // more tiles than SMs (an output head): two CTAs an SM, the start of one under the end of the other
+    if (a.M <= 16) return tiles > kSMs ? launch_stream<FORMAT, T, 16, false>(w, ws, xq, xs, a, st) : launch_stream<FORMAT, T, 16, true>(w, ws, xq, xs, a, st);
+    if (a.M <= 32) return tiles > kSMs ? launch_stream<FORMAT, T, 32, false>(w, ws, xq, xs, a, st) : launch_stream<FORMAT, T, 32, true>(w, ws, xq, xs, a, st);
+    if (a.M <= 64 && tiles <= kSMs) return launch_stream<FORMAT, T, 64, true>(w, ws, xq, xs, a, st);
     const int64_t fit = kSMs / 2, tm = (a.M + fp::PAIR_M - 1) / fp::PAIR_M;
     const auto waves = [&](int bn) { return (tm * ((a.N + bn - 1) / bn) + fit - 1) / fit; };
-    if (waves(128) * 400 < waves(256) * 600) return launch_pair<FORMAT, T, 128>(w, ws, xq, xs, a, st);
+    if (a.M <= 128) {
+        // tenths of us: what a launch costs, and a stage of K of each wave
+        const int64_t pair = (waves(128) * 27 < waves(256) * 30 ? 36 + waves(128) * stages * 27 / 10 : 39 + waves(256) * stages * 30 / 10);
+        const int splits = stream_splits(tiles, stages);
+        const int64_t stream = 20 + (tiles + kSMs - 1) / kSMs * ((splits > 1 ? 58 : 42) + stages / splits * 25 / 10);
+        if (stream <= pair) return launch_stream<FORMAT, T, 128, true>(w, ws, xq, xs, a, st);
+    }
+    if (waves(128) * 400 <= waves(256) * 600) return launch_pair<FORMAT, T, 128>(w, ws, xq, xs, a, st);
     return launch_pair<FORMAT, T, 256>(w, ws, xq, xs, a, st);
 }
 

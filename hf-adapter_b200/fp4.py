@@ -45,34 +45,38 @@ def fp4_scale_rows(scales, rows: int, blocks: int):
     return scales.permute(0, 3, 2, 1, 4).reshape(int(scales.shape[0]) * 128, -1)[:rows, :blocks].contiguous()
 
 
-def _rows2d(x, what):
+def _rows2d(x, K, what):
     """``x`` as ``[rows, K]`` whose rows the kernels can load: unit stride, 16-byte aligned (a copy where they are not)."""
-    K = int(x.shape[-1]) if x.dim() else 0
-    if K == 0 or K % 32:
+    if K <= 0 or K % 32:
         raise ValueError(f"{what}: the last dimension must be a positive multiple of 32 (got {tuple(x.shape)})")
-    x2 = x.reshape(-1, K)
-    es = x2.element_size()
-    if x2.stride(1) == 1 and (x2.shape[0] <= 1 or (x2.stride(0) >= K and x2.stride(0) * es % 16 == 0)) and x2.data_ptr() % 16 == 0:
-        return x2
-    return x2.clone(memory_format=torch.contiguous_format)
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    ld, unit = x2.stride()
+    if unit == 1 and x2.data_ptr() % 16 == 0 and (x2.shape[0] <= 1 or (ld >= K and ld * x2.element_size() % 16 == 0)):
+        return x2, ld if ld >= K else K
+    return x2.clone(memory_format=torch.contiguous_format), K
 
 
-def _ld(x2):
-    return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
+def _on_gpu(what, *tensors):
+    """All on one GPU; the checks of ``require_cuda`` by device index, which cost a call of one token less."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            require_cuda(*tensors, what=what)
 
 
 def quantize_fp4(x, format: str = "nvfp4"):
     """``x [..., K]`` (fp16 / bf16 / fp32, K a multiple of 32) to ``(packed [rows, K/2] uint8, scales, row_scale)``."""
     f = _format(format)
-    require_cuda(x, what="quantize_fp4")
+    _on_gpu("quantize_fp4", x)
     dt = dt_code(x)
-    x2 = _rows2d(x, "quantize_fp4")
-    rows, K = x2.shape
-    packed = torch.empty((rows, K // 2), device=x.device, dtype=torch.uint8)
-    scales = torch.empty(_tile_shape(rows, K, format), device=x.device, dtype=torch.uint8)
-    row_scale = torch.empty((rows,), device=x.device, dtype=torch.float32) if f else None
+    K = x.shape[-1] if x.dim() else 0
+    x2, ld = _rows2d(x, K, "quantize_fp4")
+    rows = x2.shape[0]
+    packed = x2.new_empty((rows, K // 2), dtype=torch.uint8)
+    scales = packed.new_empty(_tile_shape(rows, K, format))
+    row_scale = x2.new_empty(rows, dtype=torch.float32) if f else None
     if rows:
-        _lib.check(_lib.lib.rwkv7_fp4_quant(x2.data_ptr(), _ld(x2), packed.data_ptr(), scales.data_ptr(), ptr(row_scale), rows, K, f, dt,
+        _lib.check(_lib.lib.rwkv7_fp4_quant(x2.data_ptr(), ld, packed.data_ptr(), scales.data_ptr(), ptr(row_scale), rows, K, f, dt,
                                             stream_ptr(x2)), "quantize_fp4")
     return packed, scales, row_scale
 
@@ -111,25 +115,28 @@ def quantize_fp4_weight(weight, format: str = "nvfp4"):
 def _check_quantised(packed, scales, row_scale, format, what):
     """The kernels take their sizes from ``packed``: everything else has to hold as much."""
     f = _format(format)
-    if packed.dim() != 2 or packed.dtype != torch.uint8 or packed.shape[1] == 0 or packed.shape[1] % 16:
-        raise ValueError(f"{what}: packed must be [rows, K/2] uint8 with K a positive multiple of 32, got {tuple(packed.shape)} {packed.dtype}")
-    rows, K = packed.shape[0], 2 * packed.shape[1]
-    if scales.dtype != torch.uint8 or tuple(scales.shape) != _tile_shape(rows, K, format):
-        raise ValueError(f"{what}: scales must be uint8 tiles {_tile_shape(rows, K, format)}, got {tuple(scales.shape)} {scales.dtype}")
-    if row_scale is not None and (f == 0 or row_scale.dtype != torch.float32 or tuple(row_scale.shape) != (rows,)):
+    shape = packed.shape
+    if len(shape) != 2 or packed.dtype is not torch.uint8 or shape[1] == 0 or shape[1] % 16:
+        raise ValueError(f"{what}: packed must be [rows, K/2] uint8 with K a positive multiple of 32, got {tuple(shape)} {packed.dtype}")
+    rows, K = shape[0], 2 * shape[1]
+    tiles = _tile_shape(rows, K, format)
+    if scales.dtype is not torch.uint8 or scales.shape != tiles:
+        raise ValueError(f"{what}: scales must be uint8 tiles {tiles}, got {tuple(scales.shape)} {scales.dtype}")
+    if row_scale is not None and (f == 0 or row_scale.dtype is not torch.float32 or row_scale.shape != (rows,)):
         raise ValueError(f"{what}: row_scale must be [{rows}] float32, and None for 'mxfp4'")
-    if not packed.is_contiguous() or not scales.is_contiguous() or (row_scale is not None and not row_scale.is_contiguous()):
+    if not (packed.is_contiguous() and scales.is_contiguous() and (row_scale is None or row_scale.is_contiguous())):
         raise ValueError(f"{what}: packed, scales and row_scale must be contiguous")
     return f, rows, K
 
 
 def dequantize_fp4(packed, scales, row_scale=None, *, format: str = "nvfp4", dtype=torch.float32):
     """The values ``[rows, K]`` in ``dtype`` (formed in fp32, rounded once)."""
-    require_cuda(packed, scales, row_scale, what="dequantize_fp4")
+    _on_gpu("dequantize_fp4", packed, scales, row_scale)
     f, rows, K = _check_quantised(packed, scales, row_scale, format, "dequantize_fp4")
-    out = torch.empty((rows, K), device=packed.device, dtype=dtype)
+    out = packed.new_empty((rows, K), dtype=dtype)
+    dt = dt_code(out)
     if rows:
-        _lib.check(_lib.lib.rwkv7_fp4_dequant(packed.data_ptr(), scales.data_ptr(), ptr(row_scale), out.data_ptr(), rows, K, f, dt_code(out),
+        _lib.check(_lib.lib.rwkv7_fp4_dequant(packed.data_ptr(), scales.data_ptr(), ptr(row_scale), out.data_ptr(), rows, K, f, dt,
                                               stream_ptr(packed)), "dequantize_fp4")
     return out
 
@@ -138,32 +145,33 @@ def fp4_linear(x, packed, scales, row_scale=None, bias=None, *, format: str = "n
     """``x [..., K] @ weight.T (+ bias)`` then ``relu(.)**2`` or ``+ residual``, both operands in ``format``: ``x`` is
     quantised on the way, as ``quantize_fp4`` does it; the weight is ``quantize_fp4``'s three tensors.  Sums are fp32 and
     rounded once, after the epilogue."""
-    require_cuda(x, packed, scales, row_scale, bias, residual, out, what="fp4_linear")
+    _on_gpu("fp4_linear", x, packed, scales, row_scale, bias, residual, out)
     f, N, K = _check_quantised(packed, scales, row_scale, format, "fp4_linear")
-    if x.shape[-1] != K:
-        raise ValueError(f"fp4_linear: input must end in {K} features; got {tuple(x.shape)}")
+    shape = x.shape
+    if not shape or shape[-1] != K:
+        raise ValueError(f"fp4_linear: input must end in {K} features; got {tuple(shape)}")
     if relu2 and residual is not None:
         raise ValueError("fp4_linear: the relu^2 epilogue takes no residual")
-    dt = dt_code(x)
-    x2 = _rows2d(x, "fp4_linear")
+    dt, dtype = dt_code(x), x.dtype
+    x2, ld = _rows2d(x, K, "fp4_linear")
     M = x2.shape[0]
-    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
+    if bias is not None and (bias.dtype is not dtype or bias.shape != (N,) or not bias.is_contiguous()):
         raise ValueError(f"fp4_linear: bias must be a contiguous [{N}] in the activation dtype")
     if residual is not None:
-        if residual.dtype != x.dtype or residual.numel() != M * N:
+        if residual.dtype is not dtype or residual.numel() != M * N:
             raise ValueError(f"fp4_linear: residual must be [{M}, {N}] in the activation dtype")
-        residual = residual.reshape(M, N).contiguous()
+        if not residual.is_contiguous():
+            residual = residual.contiguous()
     if out is None:
-        out = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
-    elif out.dtype != x.dtype or out.numel() != M * N or not out.is_contiguous():
+        out = x2.new_empty((*shape[:-1], N))
+    elif out.dtype is not dtype or out.numel() != M * N or not out.is_contiguous():
         raise ValueError(f"fp4_linear: out must be a contiguous [{M}, {N}] in the activation dtype")
     if M and N:
         nbytes = _lib.lib.rwkv7_fp4_linear_workspace_bytes(M, K, f)
-        ws = torch.empty((nbytes,), device=x.device, dtype=torch.uint8)
-        epi = _lib.EPI_RELU2 if relu2 else _lib.EPI_ADD if residual is not None else _lib.EPI_NONE
-        _lib.check(_lib.lib.rwkv7_fp4_linear(x2.data_ptr(), _ld(x2), packed.data_ptr(), scales.data_ptr(), ptr(row_scale), ptr(bias),
-                                             ptr(residual), out.data_ptr(), ws.data_ptr(), nbytes, M, K, N, epi, f, dt, stream_ptr(x2)),
-                   "fp4_linear", kernels=2)
+        ws = packed.new_empty(nbytes)
+        epi = _lib.EPI_RELU2 if relu2 else _lib.EPI_NONE if residual is None else _lib.EPI_ADD
+        _lib.check(_lib.lib.rwkv7_fp4_linear(x2.data_ptr(), ld, packed.data_ptr(), scales.data_ptr(), ptr(row_scale), ptr(bias), ptr(residual),
+                                             out.data_ptr(), ws.data_ptr(), nbytes, M, K, N, epi, f, dt, stream_ptr(x2)), "fp4_linear", 2)
     return out
 
 

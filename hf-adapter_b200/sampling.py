@@ -28,76 +28,82 @@ def _vector(v, B, dtype, dev, name, keep):
     """``(pointer, value)`` of a parameter that is a number for all rows or a vector ``[B]`` on the device."""
     if not isinstance(v, torch.Tensor):
         return 0, v
-    if v.dim() != 1 or v.shape[0] != B:
+    if v.shape != (B,):
         raise ValueError(f"{name} must be a number or a vector [{B}], got {tuple(v.shape)}")
-    if v.device != dev:
-        raise ValueError(f"{name} must be on {dev}")
-    if v.dtype != dtype or not v.is_contiguous():
+    if v.get_device() != dev:
+        raise ValueError(f"{name} must be on the device of the logits")
+    if v.dtype is not dtype or not v.is_contiguous():
         v = v.to(dtype).contiguous()
-    keep.append(v)
+        keep.append(v)
     return v.data_ptr(), 0
 
 
 def _rows_of(t, B, width, name):
     """``(pointer, row stride)`` of a ``[width]`` or ``[1 | B, width]`` tensor whose rows have unit stride."""
-    if t.dim() == 1:
-        t = t[None]
-    if t.dim() != 2 or t.shape[0] not in (1, B) or t.shape[1] != width:
-        raise ValueError(f"{name} must be [{width}] or [{B}, {width}], got {tuple(t.shape)}")
-    if t.stride(1) != 1 and width > 1:
+    shape, stride = t.shape, t.stride()
+    if len(shape) not in (1, 2) or shape[-1] != width or (len(shape) == 2 and shape[0] not in (1, B)):
+        raise ValueError(f"{name} must be [{width}] or [{B}, {width}], got {tuple(shape)}")
+    if stride[-1] != 1 and width > 1:
         raise ValueError(f"{name} must have rows of unit stride")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0
+    return t.data_ptr(), stride[0] if len(shape) == 2 and shape[0] > 1 else 0
+
+
+def _rows_in(t, B, V):
+    """``t [B, V]`` with rows of unit stride that do not overlap (a copy where they do not lie so), and their distance."""
+    ld, unit = t.stride()
+    if (V > 1 and unit != 1) or (B > 1 and ld < V):
+        t = t.contiguous()
+        ld = V
+    return t, ld if B > 1 else V
 
 
 def _logits(logits, what):
-    require_cuda(logits, what=what)
-    if logits.dim() != 2 or logits.shape[1] == 0:
-        raise ValueError(f"{what}: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
+    dev = logits.get_device()
+    if dev < 0:
+        require_cuda(logits, what=what)
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"{what}: logits must be [rows, vocabulary], got {tuple(shape)}")
     dt = dt_code(logits)
-    B, V = logits.shape
-    if (V > 1 and logits.stride(1) != 1) or (B > 1 and logits.stride(0) < V):
-        logits = logits.contiguous()
-    return logits, B, V, dt
-
-
-def _ld(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    B, V = shape
+    logits, ld = _rows_in(logits, B, V)
+    return logits, ld, B, V, dt, dev
 
 
 def _rules(B, V, dev, keep, what, tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, allowed):
     r = _Rules()
     r.repetition_value = 1.0
     if tokens is not None:
-        if tokens.dim() != 2 or tokens.shape[0] != B or tokens.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{what}: tokens must be [{B}, n] int32 or int64, got {tuple(tokens.shape)} {tokens.dtype}")
-        require_cuda(tokens, lengths, prompt_lengths, what=what)
-        if tokens.device != dev:
+        shape = tokens.shape
+        if len(shape) != 2 or shape[0] != B or tokens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{what}: tokens must be [{B}, n] int32 or int64, got {tuple(shape)} {tokens.dtype}")
+        if tokens.get_device() != dev:
+            require_cuda(tokens, what=what)
             raise ValueError(f"{what}: tensors must be on the same device")
-        if tokens.shape[1]:
-            if (tokens.shape[1] > 1 and tokens.stride(1) != 1) or (B > 1 and tokens.stride(0) < tokens.shape[1]):
-                tokens = tokens.contiguous()
-            keep.append(tokens)
-            r.tokens, r.tokens_ld, r.history, r.tokens_i64 = tokens.data_ptr(), _ld(tokens), tokens.shape[1], int(tokens.dtype == torch.int64)
-            for name, v in (("lengths", lengths), ("prompt_lengths", prompt_lengths)):
-                if v is not None:
-                    setattr(r, name, _vector(v, B, torch.int32, dev, name, keep)[0])
-            for name, v in (("repetition", repetition_penalty), ("presence", presence_penalty), ("frequency", frequency_penalty)):
-                p, value = _vector(v, B, torch.float32, dev, f"{name}_penalty", keep)
-                if p:
-                    setattr(r, name, p)
-                else:
-                    if name == "repetition" and not value > 0:
-                        raise ValueError(f"{what}: repetition_penalty must be positive")
-                    setattr(r, name + "_value", value)
+        n = shape[1]
+        if n:
+            rows, r.tokens_ld = _rows_in(tokens, B, n)
+            if rows is not tokens:
+                keep.append(rows)
+            r.tokens, r.history, r.tokens_i64 = rows.data_ptr(), n, rows.dtype is torch.int64
+            if lengths is not None:
+                r.lengths = _vector(lengths, B, torch.int32, dev, "lengths", keep)[0]
+            if prompt_lengths is not None:
+                r.prompt_lengths = _vector(prompt_lengths, B, torch.int32, dev, "prompt_lengths", keep)[0]
+            if not isinstance(repetition_penalty, torch.Tensor) and not repetition_penalty > 0:
+                raise ValueError(f"{what}: repetition_penalty must be positive")
+            r.repetition, r.repetition_value = _vector(repetition_penalty, B, torch.float32, dev, "repetition_penalty", keep)
+            r.presence, r.presence_value = _vector(presence_penalty, B, torch.float32, dev, "presence_penalty", keep)
+            r.frequency, r.frequency_value = _vector(frequency_penalty, B, torch.float32, dev, "frequency_penalty", keep)
     elif lengths is not None or prompt_lengths is not None:
         raise ValueError(f"{what}: lengths need tokens")
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.device != dev:
-            raise ValueError(f"{what}: bias must be float32 on {dev}")
+        if bias.dtype is not torch.float32 or bias.get_device() != dev:
+            raise ValueError(f"{what}: bias must be float32 on the device of the logits")
         r.bias, r.bias_ld = _rows_of(bias, B, V, "bias")
     if allowed is not None:
-        if allowed.dtype != torch.int32 or allowed.device != dev:
-            raise ValueError(f"{what}: allowed must be int32 words on {dev}")
+        if allowed.dtype is not torch.int32 or allowed.get_device() != dev:
+            raise ValueError(f"{what}: allowed must be int32 words on the device of the logits")
         r.allowed, r.allowed_ld = _rows_of(allowed, B, (V + 31) // 32, "allowed")
     return r
 
@@ -112,17 +118,20 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
     presence_penalty``.  Then ``bias [V] | [B,V]`` (fp32) is added, and a token whose bit in ``allowed [ceil(V/32)] | [B,
     ceil(V/32)]`` (int32 words, token v at bit v % 32 of word v // 32) is 0 gets -inf, whatever its logit.  Penalties are numbers
     or vectors ``[B]``.  ``out`` may be ``logits``."""
-    logits, B, V, dt = _logits(logits, "process_logits")
+    logits, ld, B, V, dt, dev = _logits(logits, "process_logits")
     keep = []
-    r = _rules(B, V, logits.device, keep, "process_logits", tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty,
-               frequency_penalty, bias, allowed)
+    r = _rules(B, V, dev, keep, "process_logits", tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias,
+               allowed)
+    out_ld = V
     if out is None:
-        out = torch.empty((B, V), device=logits.device, dtype=logits.dtype)
-    elif (out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or (V > 1 and out.stride(1) != 1)
-          or (B > 1 and out.stride(0) < V)):
-        raise ValueError(f"process_logits: out must be like logits, [{B}, {V}] with rows of unit stride")
+        out = logits.new_empty((B, V))
+    else:
+        out_ld = out.stride(0) if B > 1 and out.dim() == 2 else V
+        if (out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != dev or (V > 1 and out.stride(1) != 1)
+                or out_ld < V):
+            raise ValueError(f"process_logits: out must be like logits, [{B}, {V}] with rows of unit stride")
     if B:
-        _lib.check(_lib.lib.rwkv7_process_logits(logits.data_ptr(), _ld(logits), ctypes.addressof(r), out.data_ptr(), _ld(out), B, V, dt,
+        _lib.check(_lib.lib.rwkv7_process_logits(logits.data_ptr(), ld, ctypes.addressof(r), out.data_ptr(), out_ld, B, V, dt,
                                                  stream_ptr(logits)), "process_logits")
     return out
 
@@ -141,29 +150,25 @@ def sample_tokens(logits, noise=None, *, temperature=1.0, top_k=0, top_p=1.0, mi
 
     NaN is never drawn; a row that its mask leaves empty gives -1.  The log-probability is that of softmax(z / temperature)
     after the rules, before the filters (-inf for -1)."""
-    logits, B, V, dt = _logits(logits, "sample_tokens")
-    dev, keep = logits.device, []
-    r = _rules(B, V, dev, keep, "sample_tokens", tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty,
-               bias, allowed)
-    noise_ld = 0
+    logits, ld, B, V, dt, dev = _logits(logits, "sample_tokens")
+    keep = []
+    r = _rules(B, V, dev, keep, "sample_tokens", tokens, lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias,
+               allowed)
+    noise_ptr = noise_ld = 0
     if noise is not None:
-        if noise.shape != logits.shape or noise.dtype != torch.float32 or noise.device != dev:
-            raise ValueError(f"sample_tokens: noise must be [{B}, {V}] float32 on {dev}")
-        if (V > 1 and noise.stride(1) != 1) or (B > 1 and noise.stride(0) < V):
-            noise = noise.contiguous()
-        noise_ld = _ld(noise)
+        if noise.shape != (B, V) or noise.dtype is not torch.float32 or noise.get_device() != dev:
+            raise ValueError(f"sample_tokens: noise must be [{B}, {V}] float32 on the device of the logits")
+        noise, noise_ld = _rows_in(noise, B, V)
+        noise_ptr = noise.data_ptr()
     d = _Draw()
-    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
-                           ("top_k", top_k, torch.int32)):
-        p, value = _vector(v, B, dtype, dev, name, keep)
-        if p:
-            setattr(d, name, p)
-        else:
-            setattr(d, name + "_value", value if name != "top_k" else min(int(value), 2 ** 31 - 1))
-    token = torch.empty((B,), device=dev, dtype=torch.int64)
-    logprob = torch.empty((B,), device=dev, dtype=torch.float32) if return_logprobs else None
+    d.temperature, d.temperature_value = _vector(temperature, B, torch.float32, dev, "temperature", keep)
+    d.top_p, d.top_p_value = _vector(top_p, B, torch.float32, dev, "top_p", keep)
+    d.min_p, d.min_p_value = _vector(min_p, B, torch.float32, dev, "min_p", keep)
+    d.top_k, d.top_k_value = _vector(top_k if isinstance(top_k, torch.Tensor) else min(int(top_k), 2 ** 31 - 1), B, torch.int32, dev, "top_k", keep)
+    token = logits.new_empty(B, dtype=torch.int64)
+    logprob = logits.new_empty(B, dtype=torch.float32) if return_logprobs else None
     if B:
-        _lib.check(_lib.lib.rwkv7_sample_tokens(logits.data_ptr(), _ld(logits), ctypes.addressof(r), ctypes.addressof(d),
-                                                0 if noise is None else noise.data_ptr(), noise_ld, token.data_ptr(),
-                                                0 if logprob is None else logprob.data_ptr(), B, V, dt, stream_ptr(logits)), "sample_tokens")
+        _lib.check(_lib.lib.rwkv7_sample_tokens(logits.data_ptr(), ld, ctypes.addressof(r), ctypes.addressof(d), noise_ptr, noise_ld,
+                                                token.data_ptr(), 0 if logprob is None else logprob.data_ptr(), B, V, dt, stream_ptr(logits)),
+                   "sample_tokens")
     return (token, logprob) if return_logprobs else token
