@@ -498,20 +498,23 @@ __device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, flo
 }
 
 // Every token of the window, no key beyond `limit`, to the first CTA's list; the masses (if asked for) of it and of what lies
-// above to every CTA.  Ends with a cluster barrier.
+// above to every CTA.  `few`: so few tokens that each takes its own place, else a CTA takes places for all of its at once.  Ends
+// with a cluster barrier.
 template <int VEC>
 __device__ __forceinline__ void gather(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, int stage,
-                                       unsigned int limit, bool masses) {
+                                       unsigned int limit, bool masses, bool few) {
     using lg::u64;
     const int w0 = s.window_first, w1 = s.window_last, C = cl.num_blocks(), rank = cl.block_rank();
-    u64 mine = 0;  // (tokens of the window in this slice; some may lie beyond the limit)
-    for (int b = w0 + threadIdx.x; b <= w1; b += lg::THREADS) mine += s.count[b];
-    mine = block_add(mine, s.warp_mass);
     lg::Shared* head = cl.map_shared_rank(&s, 0);
-    if (threadIdx.x == 0) s.list_base = mine ? atomicAdd(&head->list_n[stage], (unsigned int)mine) : 0, s.list_at = 0;
-    __syncthreads();
+    u64 mine = 0;  // (tokens of the window in this slice; some may lie beyond the limit)
+    if (!few) {
+        for (int b = w0 + threadIdx.x; b <= w1; b += lg::THREADS) mine += s.count[b];
+        mine = block_add(mine, s.warp_mass);
+        if (threadIdx.x == 0) s.list_base = mine ? atomicAdd(&head->list_n[stage], (unsigned int)mine) : 0, s.list_at = 0;
+        __syncthreads();
+    }
     u64 above = 0, listed = 0;
-    if (mine || (masses && w0))
+    if (few || mine || (masses && w0))
         each_token<VEC>(zs, slice, [&](int j, float z) {
             const int b = linear_bin(m, z);
             if (b > w1) return;
@@ -523,10 +526,12 @@ __device__ __forceinline__ void gather(const float* zs, int slice, int first, fl
             const unsigned int key = down_key(z);
             const bool in = key <= limit;
             if (in) listed += e;
-            head->list[s.list_base + atomicAdd(&s.list_at, 1u)] = in ? (u64)key << 32 | (unsigned int)(first + j) : ~0ull;
+            const unsigned int at = few ? atomicAdd(&head->list_n[stage], 1u) : s.list_base + atomicAdd(&s.list_at, 1u);
+            head->list[at] = in ? (u64)key << 32 | (unsigned int)(first + j) : ~0ull;
         });
     if (masses) {
-        above = block_add(above, s.warp_mass), listed = block_add(listed, s.warp_mass);
+        if (w0) above = block_add(above, s.warp_mass);
+        listed = block_add(listed, s.warp_mass);
         if ((int)threadIdx.x < C) {
             lg::Shared* o = cl.map_shared_rank(&s, threadIdx.x);
             o->mass_of[stage][0][rank] = above, o->mass_of[stage][1][rank] = listed;
@@ -541,6 +546,20 @@ __device__ __forceinline__ void sort_list(lg::u64* list, int n) {
     while (size < n) size *= 2;
     for (int i = n + threadIdx.x; i < size; i += lg::THREADS) list[i] = ~0ull;
     __syncthreads();
+    if (size <= 64) {  // one warp, a pair a lane: no barrier between the steps (50 tokens: 4600 -> 1300 cycles)
+        if (threadIdx.x < 32)
+            for (int span = 2; span <= size; span *= 2)
+                for (int d = span / 2; d > 0; d /= 2) {
+                    const int t = threadIdx.x, i = 2 * t - (t & (d - 1));
+                    if (t < size / 2) {
+                        const lg::u64 a = list[i], b = list[i + d];
+                        if ((a > b) == ((i & span) == 0)) list[i] = b, list[i + d] = a;
+                    }
+                    __syncwarp();
+                }
+        __syncthreads();
+        return;
+    }
     for (int span = 2; span <= size; span *= 2)
         for (int d = span / 2; d > 0; d /= 2) {
             for (int t = threadIdx.x; t < size / 2; t += lg::THREADS) {
@@ -777,10 +796,23 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
     if ((by_k || by_p) && m != -INFINITY) {
         // counts by distance from the largest value; every CTA sums up the bins it owns and reads the others' from their owners
         double sum = 0.0;
-        each_token<VEC>(zs, slice, [&](int, float z) {
-            atomicAdd(&s.count[linear_bin(m, z)], 1u);
-            sum += (double)fast_exp(z - m);
-        });
+        for (int j = threadIdx.x * VEC; j < slice; j += THREADS * VEC) {
+#pragma unroll
+            for (int h = 0; h < VEC; h += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
+                const float z[4] = {w.x, w.y, w.z, w.w};
+                float part = 0.0f;
+                int ones = 0;  // counted apart, as in finish()
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (z[i] != -INFINITY) atomicAdd(&s.count[linear_bin(m, z[i])], 1u);
+                    const float e = fast_exp(z[i] - m);
+                    if (e == 1.0f) ++ones;
+                    else part += e;
+                }
+                sum += (double)part + (double)ones;
+            }
+        }
         sum = block_add(sum, s.warp_sum);  // (its barriers also end the counting)
         const int per = BINS / C;
         for (int b = threadIdx.x; b < BINS; b += THREADS)
@@ -813,9 +845,12 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
             const int w0 = s.window_first, w1 = s.window_last;
             bool done = false;
             if (w0 <= w1) {
-                gather<VEC>(zs, slice, first, m, s, cl, stage, cut_k.key, by_p);
+                // (on a list that holds all that top-k keeps the first CTA finds the masses itself)
+                const bool masses = by_p && !(stage == 0 && w0 == 0);
+                const unsigned int tokens = s.upto[w1] - (w0 ? s.upto[w0 - 1] : 0);
+                gather<VEC>(zs, slice, first, m, s, cl, stage, cut_k.key, masses, tokens <= 128);
                 u64 above = 0, listed = 0;
-                for (int c = 0; by_p && c < C; ++c) above += s.mass_of[stage][0][c], listed += s.mass_of[stage][1][c];
+                for (int c = 0; masses && c < C; ++c) above += s.mass_of[stage][0][c], listed += s.mass_of[stage][1][c];
                 // (by count the window is right; by mass the exact one has to agree, or everything is on the list)
                 const bool right = stage == 0 || (above < target_p && above + listed >= target_p) || (w0 == 0 && w1 == BINS - 1);
                 if (right && w0 == 0 && rank) return;  // the first CTA has all that may be kept
