@@ -613,8 +613,19 @@ __device__ __forceinline__ int places_upto(const lg::u64* list, int n, unsigned 
     return lo;
 }
 
-// e = exp(d) for the sums and races over all tokens: one ex2, off by 2^-22 and |d| 2^-23; what decides a cut by mass uses expf
-__device__ __forceinline__ float fast_exp(float d) { return __expf(d); }
+// e = exp(d) for the sums and races over all tokens: one ex2, off by 2^-22 and |d| 2^-23 (exactly 1 at 0); what decides a cut by
+// mass uses expf
+__device__ __forceinline__ float fast_exp(float d) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.44269504f));
+    return e;
+}
+// e / q of a race, off by 2^-22: equal operands give equal scores, nearer ones are nearer than the noise is random
+__device__ __forceinline__ float race_score(float e, float q) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(q));
+    return e * r;
+}
 
 // The draw of one row, and which of its filters are on
 struct Draw {
@@ -681,34 +692,50 @@ __device__ __forceinline__ void row_max(float& m, int& top, lg::Shared& s, cg::c
 }
 
 // Sum of exponentials and the race over this CTA's tokens that `keep(key, token, e)` lets in, and the row's answer from the parts
-template <int VEC, typename F>
-__device__ __forceinline__ void finish(const float* zs, int slice, int first, float m, int top, const Draw& d, const float* q, bool sums,
+// (EVERY: all of them are likely to be let in)
+template <int VEC, bool EVERY, typename F>
+__device__ __forceinline__ void finish(const float* zs, int slice, int first, int V, float m, int top, const Draw& d, const float* q, bool sums,
                                        lg::Shared& s, cg::cluster_group& cl, long long* token, float* logprob, F keep) {
     using lg::Part;
     const int C = cl.num_blocks(), rank = cl.block_rank();
     Part best{0.0, m, -1.0f, 0.0f, top, 0x7fffffff};
+    int ones = 0;  // e = 1 is counted apart: a sure token's log-probability is all in the small terms
+    // noise by vectors where its row allows it (the tokens of a vector may begin before the row: those alone are read one by one)
+    const bool vectors = ((reinterpret_cast<uintptr_t>(q) / 4 + first) & 3) == 0;
     if ((sums || !d.greedy) && m != -INFINITY)
         for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
 #pragma unroll
             for (int h = 0; h < VEC; h += 4) {
                 const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
                 const float z[4] = {w.x, w.y, w.z, w.w};
-                float part = 0.0f;
-                int ones = 0;  // counted apart: a sure token's log-probability is all in the small terms
+                const int v0 = first + j + h;
+                float n[4] = {1.0f, 1.0f, 1.0f, 1.0f}, part = 0.0f;
+                if (EVERY && !d.greedy) {
+                    if (vectors && v0 >= 0 && v0 + 4 <= V) {
+                        const float4 t = *reinterpret_cast<const float4*>(q + v0);
+                        n[0] = t.x, n[1] = t.y, n[2] = t.z, n[3] = t.w;
+                    } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = fast_exp(z[i] - m);
-                    if (e == 1.0f) ++ones;
-                    else part += e;
-                    const int v = first + j + h + i;
-                    if (!d.greedy && z[i] != -INFINITY && keep(z[i], v, e)) {
-                        const float score = __fdividef(e, q[v]);
-                        if (score > best.score) best.score = score, best.index = v, best.z = z[i];  // (tokens come in order)
+                        for (int i = 0; i < 4; ++i)
+                            if (v0 + i >= 0 && v0 + i < V) n[i] = q[v0 + i];
                     }
                 }
-                best.sum += (double)part + (double)ones;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = fast_exp(z[i] - m);  // (0 of what is not there)
+                    if (sums) {
+                        if (e == 1.0f) ++ones;
+                        else part += e;
+                    }
+                    if (!d.greedy && z[i] != -INFINITY && keep(z[i], v0 + i, e)) {
+                        const float score = race_score(e, EVERY ? n[i] : q[v0 + i]);
+                        if (score > best.score) best.score = score, best.index = v0 + i, best.z = z[i];  // (tokens come in order)
+                    }
+                }
+                if (sums) best.sum += (double)part;
             }
         }
+    best.sum += (double)ones;
     best = block_part(best, s);
     if (threadIdx.x == 0) cl.map_shared_rank(&s, 0)->part[rank] = best;
     cl.sync();
@@ -733,7 +760,7 @@ __device__ __forceinline__ void finish(const float* zs, int slice, int first, fl
 
 // Rows without top-k and top-p
 template <typename T, bool RULES>
-__global__ void __launch_bounds__(lg::THREADS, 3) pick_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
+__global__ void __launch_bounds__(lg::THREADS, 4) pick_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
                                                               const rwkv7_draw_params draw, const float* __restrict__ noise, int64_t noise_ld,
                                                               long long* __restrict__ token, float* __restrict__ logprob, int V, int slice) {
     using namespace lg;
@@ -759,7 +786,7 @@ __global__ void __launch_bounds__(lg::THREADS, 3) pick_kernel(const T* __restric
     const bool by_min = !d.greedy && d.min_p > 0.0f;  // the largest value of the row is needed first
     if (by_min) row_max(m, top, s, cl);
     const float least = by_min ? d.min_p : 0.0f;
-    finish<VEC>(zs, slice, first, m, top, d, q, lp != nullptr, s, cl, token + row, lp, [&](float, int, float e) { return e >= least; });
+    finish<VEC, true>(zs, slice, first, V, m, top, d, q, lp != nullptr, s, cl, token + row, lp, [&](float, int, float e) { return e >= least; });
 }
 
 // Rows with top-k or top-p
@@ -796,13 +823,13 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
     if ((by_k || by_p) && m != -INFINITY) {
         // counts by distance from the largest value; every CTA sums up the bins it owns and reads the others' from their owners
         double sum = 0.0;
+        int ones = 0;  // counted apart, as in finish()
         for (int j = threadIdx.x * VEC; j < slice; j += THREADS * VEC) {
 #pragma unroll
             for (int h = 0; h < VEC; h += 4) {
                 const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
                 const float z[4] = {w.x, w.y, w.z, w.w};
                 float part = 0.0f;
-                int ones = 0;  // counted apart, as in finish()
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (z[i] != -INFINITY) atomicAdd(&s.count[linear_bin(m, z[i])], 1u);
@@ -810,10 +837,10 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
                     if (e == 1.0f) ++ones;
                     else part += e;
                 }
-                sum += (double)part + (double)ones;
+                sum += (double)part;
             }
         }
-        sum = block_add(sum, s.warp_sum);  // (its barriers also end the counting)
+        sum = block_add(sum + (double)ones, s.warp_sum);  // (its barriers also end the counting)
         const int per = BINS / C;
         for (int b = threadIdx.x; b < BINS; b += THREADS)
             if (s.count[b]) atomicAdd(&cl.map_shared_rank(&s, b / per)->owned[b], s.count[b]);
@@ -870,7 +897,7 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
                         for (int i = 0; i < 2; ++i) {
                             if (i0 + i < kept && before < target && o.e[i] >= (d.min_p > 0.0f ? d.min_p : 0.0f)) {
                                 const int v = (int)(unsigned int)s.list[i0 + i];
-                                const float score = __fdividef(o.e[i], q[v]);
+                                const float score = race_score(o.e[i], q[v]);
                                 if (better(score, v, best.score, best.index)) best.score = score, best.index = v, best.z = o.z[i];
                             }
                             before += o.w[i];
@@ -913,7 +940,7 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
     }
     const unsigned int key = cut_k.key < cut_p.key ? cut_k.key : cut_p.key;
     const float least = d.min_p > 0.0f ? d.min_p : 0.0f;
-    finish<VEC>(zs, slice, first, m, top, d, q, logprob != nullptr, s, cl, token + row, logprob ? logprob + row : nullptr,
+    finish<VEC, false>(zs, slice, first, V, m, top, d, q, logprob != nullptr, s, cl, token + row, logprob ? logprob + row : nullptr,
                 [&](float z, int v, float e) {
                     const unsigned int kk = down_key(z);
                     return kk <= key && e >= least && !(kk == cut_p.key && v >= cut_p.index);
@@ -960,14 +987,20 @@ extern "C" int rwkv7_sample_tokens(const void* logits, int64_t ld, const rwkv7_l
     RWKV7_REQUIRE(dtype >= RWKV7_F16 && dtype <= RWKV7_F32, RWKV7_ERR_INVALID, "sample_tokens: unknown dtype %d", dtype);
     if (int e = check_rules("sample_tokens", rules)) return e;
     const int vec = 16 / (int)dtype_size(dtype);
-    int C = 1;
-    while (C < MAX_CLUSTER && V > 4096 * C) C *= 2;
-    const int64_t places = (int64_t)V + vec - 1;  // a row may begin up to vec - 1 places into its first vector
-    const int64_t slice = ((places + C - 1) / C + vec - 1) / vec * vec;
     const bool filters = noise && (draw->top_k || (draw->top_k_value > 0 && draw->top_k_value < V) || draw->top_p || draw->top_p_value < 1.0f);
+    // CTAs a row: 4096 tokens each at least, eight for the shortest way (one row, 65536 tokens, 2 / 4 / 8 us: largest logit 7.4 / 5.3 / 4.4,
+    // top-p 24 / 18.6 / 15.3).  Where the rows fill the GPU all the same, half as many larger slices cost less, the barriers being
+    // most of a CTA's time: 64 rows top-p 24.5 / 24.0 / 40.8, 256 rows 95 / 84 / 128, largest logit 28.9 / 20.6 / 29.8.  Not so the draw from
+    // every token, which is bound by its instructions: 64 rows 16.2 / 20.1 / 13.9, 256 rows 77 / 63 / 50.
+    const int most = (filters || !noise) && B > 32 ? MAX_CLUSTER / 2 : MAX_CLUSTER;
+    const int64_t places = (int64_t)V + vec - 1, shared = filters ? FILTER_SHARED : PICK_SHARED;  // a row may begin up to vec - 1 places into its first vector
+    const auto slice_of = [&](int c) { return ((places + c - 1) / c + vec - 1) / vec * vec; };
+    const auto fits = [&](int c) { return shared + slice_of(c) * 4 <= 227 * 1024; };
+    int C = 1;
+    while ((C < most && V > 4096 * C) || (C < MAX_CLUSTER && !fits(C))) C *= 2;
+    const int64_t slice = slice_of(C), smem = shared + slice * 4;
     const bool ruled = rules->tokens || rules->bias || rules->allowed;
-    const int64_t smem = (filters ? FILTER_SHARED : PICK_SHARED) + slice * 4;
-    RWKV7_REQUIRE(smem <= 227 * 1024, RWKV7_ERR_UNSUPPORTED, "sample_tokens: a vocabulary of %d tokens does not fit the shared memory of a cluster", V);
+    RWKV7_REQUIRE(fits(C), RWKV7_ERR_UNSUPPORTED, "sample_tokens: a vocabulary of %d tokens does not fit the shared memory of a cluster", V);
     RWKV7_REQUIRE((int64_t)B * C < (1ll << 31), RWKV7_ERR_UNSUPPORTED, "sample_tokens: too many rows (%d)", B);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     RWKV7_DISPATCH_DTYPE(dtype, T, {
