@@ -691,53 +691,11 @@ __device__ __forceinline__ void row_max(float& m, int& top, lg::Shared& s, cg::c
         if (better(s.max[c], s.top[c], m, top)) m = s.max[c], top = s.top[c];
 }
 
-// Sum of exponentials and the race over this CTA's tokens that `keep(key, token, e)` lets in, and the row's answer from the parts
-// (EVERY: all of them are likely to be let in)
-template <int VEC, bool EVERY, typename F>
-__device__ __forceinline__ void finish(const float* zs, int slice, int first, int V, float m, int top, const Draw& d, const float* q, bool sums,
-                                       lg::Shared& s, cg::cluster_group& cl, long long* token, float* logprob, F keep) {
+// The row's answer from the parts of its CTAs (valid in thread 0)
+__device__ __forceinline__ void answer(const lg::Part& mine, bool greedy, lg::Shared& s, cg::cluster_group& cl, long long* token, float* logprob) {
     using lg::Part;
     const int C = cl.num_blocks(), rank = cl.block_rank();
-    Part best{0.0, m, -1.0f, 0.0f, top, 0x7fffffff};
-    int ones = 0;  // e = 1 is counted apart: a sure token's log-probability is all in the small terms
-    // noise by vectors where its row allows it (the tokens of a vector may begin before the row: those alone are read one by one)
-    const bool vectors = ((reinterpret_cast<uintptr_t>(q) / 4 + first) & 3) == 0;
-    if ((sums || !d.greedy) && m != -INFINITY)
-        for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
-#pragma unroll
-            for (int h = 0; h < VEC; h += 4) {
-                const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
-                const float z[4] = {w.x, w.y, w.z, w.w};
-                const int v0 = first + j + h;
-                float n[4] = {1.0f, 1.0f, 1.0f, 1.0f}, part = 0.0f;
-                if (EVERY && !d.greedy) {
-                    if (vectors && v0 >= 0 && v0 + 4 <= V) {
-                        const float4 t = *reinterpret_cast<const float4*>(q + v0);
-                        n[0] = t.x, n[1] = t.y, n[2] = t.z, n[3] = t.w;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (v0 + i >= 0 && v0 + i < V) n[i] = q[v0 + i];
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = fast_exp(z[i] - m);  // (0 of what is not there)
-                    if (sums) {
-                        if (e == 1.0f) ++ones;
-                        else part += e;
-                    }
-                    if (!d.greedy && z[i] != -INFINITY && keep(z[i], v0 + i, e)) {
-                        const float score = race_score(e, EVERY ? n[i] : q[v0 + i]);
-                        if (score > best.score) best.score = score, best.index = v0 + i, best.z = z[i];  // (tokens come in order)
-                    }
-                }
-                if (sums) best.sum += (double)part;
-            }
-        }
-    best.sum += (double)ones;
-    best = block_part(best, s);
-    if (threadIdx.x == 0) cl.map_shared_rank(&s, 0)->part[rank] = best;
+    if (threadIdx.x == 0) cl.map_shared_rank(&s, 0)->part[rank] = mine;
     cl.sync();
     if (rank == 0 && threadIdx.x < 32) {
         Part x = s.part[threadIdx.x % C];
@@ -751,45 +709,163 @@ __device__ __forceinline__ void finish(const float* zs, int slice, int first, in
         warp_best(x.score, x.index, x.z);
         if (threadIdx.x == 0) {
             // (noise of NaN alone: the most likely token)
-            const bool empty = most == -INFINITY, drawn = !d.greedy && x.index != 0x7fffffff;
+            const bool empty = most == -INFINITY, drawn = !greedy && x.index != 0x7fffffff;
             *token = empty ? -1 : drawn ? x.index : at;
             if (logprob) *logprob = empty ? -INFINITY : ((drawn ? x.z : most) - most) - log_sum(sum);
         }
     }
 }
 
-// Rows without top-k and top-p
+// Sum of exponentials and the race over this CTA's tokens that `keep(key, token, e)` lets in, and the row's answer from the parts
+template <int VEC, typename F>
+__device__ __forceinline__ void finish(const float* zs, int slice, int first, float m, int top, const Draw& d, const float* q, bool sums,
+                                       lg::Shared& s, cg::cluster_group& cl, long long* token, float* logprob, F keep) {
+    using lg::Part;
+    Part best{0.0, m, -1.0f, 0.0f, top, 0x7fffffff};
+    int ones = 0;  // e = 1 is counted apart: a sure token's log-probability is all in the small terms
+    if ((sums || !d.greedy) && m != -INFINITY)
+        for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
+#pragma unroll
+            for (int h = 0; h < VEC; h += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
+                const float z[4] = {w.x, w.y, w.z, w.w};
+                const int v0 = first + j + h;
+                float part = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = fast_exp(z[i] - m);  // (0 of what is not there)
+                    if (sums) {
+                        if (e == 1.0f) ++ones;
+                        else part += e;
+                    }
+                    if (!d.greedy && z[i] != -INFINITY && keep(z[i], v0 + i, e)) {
+                        const float score = race_score(e, q[v0 + i]);
+                        if (score > best.score) best.score = score, best.index = v0 + i, best.z = z[i];  // (tokens come in order)
+                    }
+                }
+                if (sums) best.sum += (double)part;
+            }
+        }
+    best.sum += (double)ones;
+    best = block_part(best, s);
+    answer(best, d.greedy, s, cl, token, logprob);
+}
+
+// Rows without any filter: one pass over logits and noise, everything relative to the largest value that a thread has met so far
 template <typename T, bool RULES>
-__global__ void __launch_bounds__(lg::THREADS, 4) pick_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
+__global__ void __launch_bounds__(lg::THREADS, 2) pick_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
                                                               const rwkv7_draw_params draw, const float* __restrict__ noise, int64_t noise_ld,
                                                               long long* __restrict__ token, float* __restrict__ logprob, int V, int slice) {
     using namespace lg;
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
-    float* zs = reinterpret_cast<float*>(smem + PICK_SHARED);
+    unsigned int* words = reinterpret_cast<unsigned int*>(smem + PICK_SHARED);  // the slice's history, where there is one
     cg::cluster_group cl = cg::this_cluster();
     constexpr int VEC = 16 / sizeof(T);
+    const int rank = cl.block_rank();
     const int64_t row = blockIdx.x / cl.num_blocks();
     const T* in = logits + row * ld;
-    const int first = cl.block_rank() * slice - (int)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % VEC);
+    const int first = rank * slice - (int)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % VEC);
     cluster_arrive_relaxed();  // this CTA runs: the others may write into its shared memory
     grid_dependency_wait();
     grid_launch_dependents();
-    const Draw d = row_draw(draw, noise != nullptr, row, V);
-    float m;
-    int top;
-    load_row<T, RULES>(in, first, V, slice, rules, row, d, zs, m, top);
+    const float temperature = noise ? param(draw.temperature, draw.temperature_value, row) : 0.0f;
+    const bool greedy = !(temperature > 0.0f), sums = logprob != nullptr;
+    const float t = greedy ? 1.0f : temperature, inv = __frcp_rn(t);
+    const float* q = greedy ? nullptr : noise + row * noise_ld;
+    const bool vectors = ((reinterpret_cast<uintptr_t>(q) / 4 + first) & 3) == 0;
+    Row r{};
+    if constexpr (RULES) {
+        r = row_rules(rules, row);
+        if (r.history) count_history(rules, row, first, slice, words);
+    }
+    Part x{0.0, -INFINITY, 0.0f, 0.0f, 0x7fffffff, 0x7fffffff};  // (a token's score is positive, that of a masked one 0)
+    float small = 0.0f;
+    int ones = 0;  // e = 1 is counted apart: a sure token's log-probability is all in the small terms
+    constexpr int TOK = 8;  // tokens a turn
+#pragma unroll 2
+    for (int j = threadIdx.x * TOK; j < slice; j += THREADS * TOK) {
+        const int v0 = first + j;
+        if (v0 >= V) break;
+        float z[TOK], n[TOK];
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) n[i] = 1.0f;
+        if (!greedy) {
+            if (vectors && v0 >= 0 && v0 + TOK <= V) {
+#pragma unroll
+                for (int h = 0; h < TOK; h += 4) {
+                    const float4 w = *reinterpret_cast<const float4*>(q + v0 + h);
+                    n[h] = w.x, n[h + 1] = w.y, n[h + 2] = w.z, n[h + 3] = w.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < TOK; ++i)
+                    if (v0 + i >= 0 && v0 + i < V) n[i] = q[v0 + i];
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < TOK; h += VEC) {
+            float part[VEC];
+            load_vector<T, VEC, RULES>(in, v0 + h, V, r, words + j + h, part);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) z[h + i] = part[i];
+        }
+        // over_temperature() with one branch a turn
+        float a[TOK], most = -INFINITY;
+        bool plain = true;
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) a[i] = z[i] * inv, plain = plain && fabsf(a[i]) < 1e37f;
+        if (plain) {
+#pragma unroll
+            for (int i = 0; i < TOK; ++i) z[i] = fmaf(fmaf(-a[i], t, z[i]), inv, a[i]);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < TOK; ++i) {
+                float y = 0.0f;
+#pragma unroll
+                for (int k = 0; k < TOK; ++k) y = k == i ? z[k] : y;  // (no indexed registers)
+                y = over_temperature(y, t, inv);
+#pragma unroll
+                for (int k = 0; k < TOK; ++k) z[k] = k == i ? y : z[k];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) most = fmaxf(most, z[i]);
+        if (most > x.max) {
+            const float f = fast_exp(x.max - most);  // (0 the first time)
+            x.score *= f, small = (small + (float)ones) * f, ones = 0;
+            x.max = most;
+#pragma unroll
+            for (int i = TOK - 1; i >= 0; --i)
+                if (z[i] == most) x.top = v0 + i;  // (the first of them)
+        }
+        if ((greedy && !sums) || x.max == -INFINITY) continue;
+#pragma unroll
+        for (int i = 0; i < TOK; ++i) {
+            const float e = fast_exp(z[i] - x.max);  // (0 of what is masked or not there)
+            if (sums) {
+                if (e == 1.0f) ++ones;
+                else small += e;
+            }
+            const float score = race_score(e, n[i]);
+            if (score > x.score) x.score = score, x.index = v0 + i, x.z = z[i];  // (tokens come in order)
+        }
+    }
+    x.sum = (double)ones + (double)small;
+    if (x.index == 0x7fffffff) x.score = -1.0f;
+    // the CTA's, relative to its largest value
+    float m = x.max;
+    int top = x.top;
     block_max_index(m, top, s);
+    const float f = x.max == -INFINITY ? 0.0f : expf(x.max - m);
+    x.sum *= (double)f, x.max = m, x.top = top;
+    if (x.index != 0x7fffffff) x.score *= f;
+    x = block_part(x, s);
     cluster_wait();
-    const float* q = noise + row * noise_ld;
-    float* lp = logprob ? logprob + row : nullptr;
-    const bool by_min = !d.greedy && d.min_p > 0.0f;  // the largest value of the row is needed first
-    if (by_min) row_max(m, top, s, cl);
-    const float least = by_min ? d.min_p : 0.0f;
-    finish<VEC, true>(zs, slice, first, V, m, top, d, q, lp != nullptr, s, cl, token + row, lp, [&](float, int, float e) { return e >= least; });
+    answer(x, greedy, s, cl, token + row, sums ? logprob + row : nullptr);
 }
 
-// Rows with top-k or top-p
+// Rows with filters
 template <typename T, bool RULES>
 __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
                                                                 const rwkv7_draw_params draw, const float* __restrict__ noise, int64_t noise_ld,
@@ -940,7 +1016,7 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
     }
     const unsigned int key = cut_k.key < cut_p.key ? cut_k.key : cut_p.key;
     const float least = d.min_p > 0.0f ? d.min_p : 0.0f;
-    finish<VEC, false>(zs, slice, first, V, m, top, d, q, logprob != nullptr, s, cl, token + row, logprob ? logprob + row : nullptr,
+    finish<VEC>(zs, slice, first, m, top, d, q, logprob != nullptr, s, cl, token + row, logprob ? logprob + row : nullptr,
                 [&](float z, int v, float e) {
                     const unsigned int kk = down_key(z);
                     return kk <= key && e >= least && !(kk == cut_p.key && v >= cut_p.index);
@@ -987,18 +1063,20 @@ extern "C" int rwkv7_sample_tokens(const void* logits, int64_t ld, const rwkv7_l
     RWKV7_REQUIRE(dtype >= RWKV7_F16 && dtype <= RWKV7_F32, RWKV7_ERR_INVALID, "sample_tokens: unknown dtype %d", dtype);
     if (int e = check_rules("sample_tokens", rules)) return e;
     const int vec = 16 / (int)dtype_size(dtype);
-    const bool filters = noise && (draw->top_k || (draw->top_k_value > 0 && draw->top_k_value < V) || draw->top_p || draw->top_p_value < 1.0f);
-    // CTAs a row: 4096 tokens each at least, eight for the shortest way (one row, 65536 tokens, 2 / 4 / 8 us: largest logit 7.4 / 5.3 / 4.4,
-    // top-p 24 / 18.6 / 15.3).  Where the rows fill the GPU all the same, half as many larger slices cost less, the barriers being
-    // most of a CTA's time: 64 rows top-p 24.5 / 24.0 / 40.8, 256 rows 95 / 84 / 128, largest logit 28.9 / 20.6 / 29.8.  Not so the draw from
-    // every token, which is bound by its instructions: 64 rows 16.2 / 20.1 / 13.9, 256 rows 77 / 63 / 50.
-    const int most = (filters || !noise) && B > 32 ? MAX_CLUSTER / 2 : MAX_CLUSTER;
+    const bool filters = noise && (draw->top_k || (draw->top_k_value > 0 && draw->top_k_value < V) || draw->top_p || draw->top_p_value < 1.0f ||
+                                   draw->min_p || draw->min_p_value > 0.0f);
+    // CTAs a row: 4096 tokens each at least, eight for the shortest way.  Where the rows fill the GPU all the same, fewer and larger
+    // slices cost less: a CTA's barriers and reductions are as long as its tokens.  us, 65536 tokens, 2 / 4 / 8 CTAs, top-p: one row 24 / 18.6 /
+    // 15.3, 64 24.5 / 24.0 / 40.8, 256 95 / 84 / 128; without filters: one row 12.9 / 8.4 / 6.1, 16 13.4 / 8.7 / 7.3, 64 13.5 / 10.9 /
+    // 14.4, 256 36.0 / 43.2 / 57.5.
+    const int most = B <= 32 ? MAX_CLUSTER : filters || B <= 100 ? MAX_CLUSTER / 2 : MAX_CLUSTER / 4;
     const int64_t places = (int64_t)V + vec - 1, shared = filters ? FILTER_SHARED : PICK_SHARED;  // a row may begin up to vec - 1 places into its first vector
-    const auto slice_of = [&](int c) { return ((places + c - 1) / c + vec - 1) / vec * vec; };
-    const auto fits = [&](int c) { return shared + slice_of(c) * 4 <= 227 * 1024; };
+    const auto slice_of = [&](int c) { return ((places + c - 1) / c + 7) / 8 * 8; };
+    const bool kept = filters || rules->tokens;  // whether a slice takes its place in shared memory
+    const auto fits = [&](int c) { return shared + slice_of(c) * 4 <= 227 * 1024; };  // (one limit for every form of the call)
     int C = 1;
     while ((C < most && V > 4096 * C) || (C < MAX_CLUSTER && !fits(C))) C *= 2;
-    const int64_t slice = slice_of(C), smem = shared + slice * 4;
+    const int64_t slice = slice_of(C), smem = shared + (kept ? slice * 4 : 0);
     const bool ruled = rules->tokens || rules->bias || rules->allowed;
     RWKV7_REQUIRE(fits(C), RWKV7_ERR_UNSUPPORTED, "sample_tokens: a vocabulary of %d tokens does not fit the shared memory of a cluster", V);
     RWKV7_REQUIRE((int64_t)B * C < (1ll << 31), RWKV7_ERR_UNSUPPORTED, "sample_tokens: too many rows (%d)", B);
