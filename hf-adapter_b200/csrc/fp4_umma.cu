@@ -69,6 +69,12 @@ __device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
 template <int GROUP> __device__ __forceinline__ void copy_scale_tile(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::%2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc), "n"(GROUP) : "memory");
 }
+// relu(y)^2, NaN stays
+__device__ __forceinline__ float relu_squared(float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(y));
+    return r * r;
+}
 __device__ __forceinline__ bool elect_lane() {  // (the compiler knows that one thread runs what this guards)
     uint32_t pred;
     asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}" : "=r"(pred));
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
     T* out = static_cast<T*>(p.y) + (size_t)m0 * p.N + n;
     const auto result = [&](float sum, int t, float r) {
         float y = fmaf(sum, gw * s_xg[t], bias);
-        if (p.relu2) y = y > 0.0f ? y * y : y != y ? y : 0.0f;
+        if (p.relu2) y = relu_squared(y);
         out[(size_t)t * p.N] = from_f<T>(y + r);
     };
 
@@ -320,9 +326,27 @@ __device__ __forceinline__ void fp4_tile(int tile, int tiles_m, int tiles_n, int
     tm = band * fp::GROUP_M + (within - tn * rows);
 }
 
+// The residual of 64 columns of a warp's 32 rows on its way into the warp's staging tile (16-bit types, aligned rows), eight lanes a
+// row, whole lines; zeros where there is none.  The last copy out of the tile is awaited before.
+__device__ __forceinline__ void request_residual(const Fp4Args& p, int row0, int col0, int lane, unsigned char* stg) {
+    if (row0 >= p.M || col0 >= p.N) return;  // (nobody would wait for it before the next request)
+    if (lane == 0) tma_store_wait_read<0>();
+    __syncwarp();
+    const int col = col0 + (lane & 7) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = (lane >> 3) + 4 * i, row = row0 + r;
+        const bool here = row < p.M && col < p.N;
+        const uint16_t* src = static_cast<const uint16_t*>(p.residual) + (here ? (size_t)row * p.N + col : 0);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     ::"r"(smem_u32(stg + r * 128 + (((lane & 7) ^ (r & 7)) << 4))), "l"(src), "r"(here ? 16 : 0) : "memory");
+    }
+}
+
 // 64 columns of a warp's 32 rows (a lane is a row): factors and bias, then MODE 0 nothing, 1 relu^2, 2 + residual.  16-bit
 // results go through the warp's staging tile (16-byte pieces xored by the row: the layout of a 128-byte-swizzled tensor map) and
-// leave as one bulk copy, or, where rows of y are not 16-byte aligned, as coalesced single values.
+// leave as one bulk copy, or, where rows of y are not 16-byte aligned, as coalesced single values.  The residual
+// comes in by the same tile (request_residual): a lane that reads its own row from memory touches 32 lines an instruction.
 template <int FORMAT, typename T, int MODE>
 __device__ __forceinline__ void fp4_columns(const Fp4Args& p, const CUtensorMap& tm_y, const uint32_t (&v)[64], const float* wg, const float* bias, float gx,
                                             int row0, int col0, int lane, unsigned char* stg) {
@@ -330,14 +354,17 @@ __device__ __forceinline__ void fp4_columns(const Fp4Args& p, const CUtensorMap&
     const size_t o = (size_t)row * p.N + col0;
     const T* res = static_cast<const T*>(p.residual) + o;
     if (sizeof(T) == 2) {
-        if (p.vec && lane == 0) tma_store_wait_read<0>();  // the last group's copy has left the staging tile
+        if (MODE == 2 && p.vec) asm volatile("cp.async.wait_all;" ::: "memory");
+        else if (p.vec && lane == 0) tma_store_wait_read<0>();  // the last group's copy has left the staging tile
         __syncwarp();
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
         float f[8], r[8];
         if constexpr (MODE == 2) {
-            if (p.vec) {
+            if (sizeof(T) == 2 && p.vec) {
+                load8<T>(reinterpret_cast<const T*>(stg + lane * 128 + ((u ^ (lane & 7)) << 4)), r);
+            } else if (p.vec) {
                 if (8 * u < live) load8<T>(res + 8 * u, r);
             } else {
 #pragma unroll
@@ -359,7 +386,7 @@ __device__ __forceinline__ void fp4_columns(const Fp4Args& p, const CUtensorMap&
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if constexpr (MODE == 1) f[e] = f[e] > 0.0f ? f[e] * f[e] : f[e] != f[e] ? f[e] : 0.0f;
+            if constexpr (MODE == 1) f[e] = relu_squared(f[e]);
             if constexpr (MODE == 2) f[e] += r[e];
         }
         if constexpr (sizeof(T) == 2) {
@@ -509,6 +536,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp::THREADS, 1) fp4_
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const int row0 = tm * PAIR_M + (int)rank * BM + q * 32, row = row0 + lane;
             const float gx = p.xg && row < p.M ? p.xg[row] : 1.0f;
+            const bool staged = sizeof(T) == 2 && p.residual && p.vec;
+            if (staged) request_residual(p, row0, tn * BN + half * GROUPS * 64, lane, stg);
             bool ok = true;
             if (lane == 0) ok = mbar_wait(&acc_full[as], (li / ACCS) & 1, actx, kErrWaitDFull);
             ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -533,6 +562,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(fp::THREADS, 1) fp4_
                 if (p.relu2) fp4_columns<FORMAT, T, 1>(p, maps.y, v[g], s_wg + c0, s_bias + c0, gx, row0, col0, lane, stg);
                 else if (p.residual) fp4_columns<FORMAT, T, 2>(p, maps.y, v[g], s_wg + c0, s_bias + c0, gx, row0, col0, lane, stg);
                 else fp4_columns<FORMAT, T, 0>(p, maps.y, v[g], s_wg + c0, s_bias + c0, gx, row0, col0, lane, stg);
+                if (staged && g + 1 < GROUPS) request_residual(p, row0, col0 + 64, lane, stg);
             }
         }
         if (lane == 0) tma_store_wait_all();
