@@ -250,10 +250,10 @@ static int quant(const void* x, int64_t ldx, uint8_t* packed, uint8_t* scales, f
     const int ktiles = k_tiles(K, FORMAT);
     const int pieces = ktiles * SCALE_TILE_BLOCKS * block_of(FORMAT) / 16;
     // Few rows: a piece a thread, for the shortest way.  Many rows: four, and several rows a CTA.  (FIXME)
-    const int per = rows >= 512 ? 4 : 1;
+    const int per = rows >= 2048 ? 4 : 1;
     int team = 32;
     while (team < 256 && team * per < pieces) team *= 2;
-    const int threads = rows >= 512 ? 256 : team;
+    const int threads = rows >= 2048 ? 256 : team;
     const int64_t all = ((int64_t)rows + SCALE_TILE_ROWS - 1) / SCALE_TILE_ROWS * SCALE_TILE_ROWS, grid = all / (threads / team);
     auto kernel = pieces <= team ? fp4_quant_kernel<T, FORMAT, 1> : pieces <= 2 * team ? fp4_quant_kernel<T, FORMAT, 2>
                   : pieces <= 4 * team ? fp4_quant_kernel<T, FORMAT, 4> : fp4_quant_kernel<T, FORMAT, 0>;

@@ -49,7 +49,7 @@ struct Shared {
     Part part[MAX_CLUSTER];           // first CTA: of every CTA
     Part warp_part[WARPS];
     double sum_of[MAX_CLUSTER];
-    u64 mass_of[2][2][MAX_CLUSTER];   // [top-k, top-p][of the tokens above the window, of those on the list]
+    u64 mass_of[4][2][MAX_CLUSTER];   // [list][of the tokens above the window, of those on the list]
     u64 warp_mass[WARPS];
     double warp_sum[WARPS];
     Cut cut[2];
@@ -60,7 +60,7 @@ struct Shared {
     unsigned int count[BINS];         // this CTA's histogram
     unsigned int owned[BINS];         // the cluster's, for the bins that this CTA owns (the others' places stay unused)
     unsigned int upto[BINS];          // the cluster's, summed from bin 0
-    unsigned int list_n[2];           // first CTA: places given out
+    unsigned int list_n[4];           // first CTA: places given out on a list: top-k's, its second try, top-p's, its second try
     unsigned int list_base, list_at;
     int bin, window_first, window_last;
     int place;
@@ -69,6 +69,7 @@ struct Shared {
         struct {         // the descent
             unsigned int count[BINS], all_count[BINS];
             u64 mass[BINS], all_mass[BINS];
+            u64 above_of[2][MAX_CLUSTER];  // [count, mass] of what lies above the range
             unsigned int ties[MAX_CLUSTER];
             unsigned int above_count, bin_count;
             u64 above_mass, bin_mass;
@@ -230,19 +231,6 @@ __device__ __forceinline__ unsigned int down_key(float z) {
     return b & 0x80000000u ? b : ~(b | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(unsigned int k) { return __uint_as_float(k & 0x80000000u ? k : ~(k | 0x80000000u)); }
-// the last key of bins 0 .. bin: linear_bin rises with the key, so a bisection between keys on both sides of the edge (the
-// bin's rounded edge is off by less than 2^-22 of the operands) finds it exactly
-__device__ __forceinline__ unsigned int last_key(float m, int bin) {
-    if (bin == lg::BINS - 1) return down_key(-lg::FLOAT_MAX);
-    const float edge = m - (float)(bin + 1) / lg::BIN_SCALE, slack = (fabsf(m) + 64.0f) * 1e-6f;
-    unsigned int lo = down_key(fminf(m, edge + slack)), hi = down_key(fmaxf(edge - slack, -lg::FLOAT_MAX));
-    while (lo < hi) {
-        const unsigned int mid = lo + (hi - lo + 1) / 2;
-        if (linear_bin(m, key_value(mid)) <= bin) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
 __device__ __forceinline__ lg::u64 fixed_mass(float e) { return __float2ull_rn(e * lg::MASS_UNIT); }
 __device__ __forceinline__ lg::u64 share_of(double share, double mass) {
     const double want = ceil(share * mass);
@@ -322,22 +310,50 @@ __device__ __forceinline__ lg::Part block_part(lg::Part x, lg::Shared& s) {
 }
 
 // ------------------------------ the descent: any number of equal or neighbouring values at a cut
-// the cluster's histogram of counts and masses over `bin_of(z)` (negative: not counted) into every CTA
-template <typename F>
-__device__ __forceinline__ void histogram(const float* zs, int slice, float m, lg::Shared& s, cg::cluster_group& cl, F bin_of) {
+// The cluster's histogram of counts and masses over `bin_of(z)` into every CTA; with ABOVE also count and mass of what it puts at -1
+// (other values outside 0 .. BINS - 1 are left out).  Equal bins of a whole warp are added up first: a row of one value would queue
+// at one address.
+template <bool ABOVE, typename F>
+__device__ __forceinline__ void histogram(const float* zs, int slice, float m, lg::Shared& s, cg::cluster_group& cl, lg::u64& above_count,
+                                          lg::u64& above_mass, F bin_of) {
+    const int C = cl.num_blocks(), rank = cl.block_rank(), per = lg::BINS / C, lane = threadIdx.x & 31;
     for (int b = threadIdx.x; b < lg::BINS; b += lg::THREADS) s.w.count[b] = 0, s.w.mass[b] = 0;
     __syncthreads();
-    for (int j = threadIdx.x; j < slice; j += lg::THREADS) {
-        const float z = zs[j];
-        if (z == -INFINITY) continue;
-        const int b = bin_of(z);
-        if (b >= 0) {
+    lg::u64 n_above = 0, q_above = 0;
+    for (int j0 = threadIdx.x - lane; j0 < slice; j0 += lg::THREADS) {
+        const int j = j0 + lane;
+        const float z = j < slice ? zs[j] : -INFINITY;
+        int b = lg::BINS;
+        lg::u64 q = 0;
+        if (z != -INFINITY) {
+            b = bin_of(z);
+            if (b < lg::BINS) q = fixed_mass(expf(z - m));
+            if (ABOVE && b < 0) ++n_above, q_above += q;
+        }
+        const bool in = b >= 0 && b < lg::BINS;
+        const int most = __reduce_max_sync(0xffffffffu, in ? b : -1);
+        if (most < 0) continue;
+        const unsigned int who = __ballot_sync(0xffffffffu, in);
+        if (__all_sync(0xffffffffu, !in || b == most)) {
+            q = warp_add(in ? q : 0);
+            if (lane == 0) atomicAdd(&s.w.count[most], (unsigned int)__popc(who)), atomicAdd(&s.w.mass[most], q);
+        } else if (in) {
             atomicAdd(&s.w.count[b], 1u);
-            atomicAdd(&s.w.mass[b], fixed_mass(expf(z - m)));
+            atomicAdd(&s.w.mass[b], q);
+        }
+    }
+    if (ABOVE) {
+        n_above = block_add(n_above, s.warp_mass), q_above = block_add(q_above, s.warp_mass);
+        if ((int)threadIdx.x < C) {
+            lg::Shared* o = cl.map_shared_rank(&s, threadIdx.x);
+            o->w.above_of[0][rank] = n_above, o->w.above_of[1][rank] = q_above;
         }
     }
     cl.sync();
-    const int C = cl.num_blocks(), rank = cl.block_rank(), per = lg::BINS / C;
+    if (ABOVE) {
+        above_count = above_mass = 0;
+        for (int c = 0; c < C; ++c) above_count += s.w.above_of[0][c], above_mass += s.w.above_of[1][c];
+    }
     for (int b = rank * per + threadIdx.x; b < (rank + 1) * per; b += lg::THREADS) {
         unsigned int n = 0;
         lg::u64 q = 0;
@@ -416,46 +432,93 @@ __device__ __forceinline__ int tie_cut(const float* zs, int slice, int first, un
     return s.w.index_cut;
 }
 
-// The key at which the descending order reaches `target` tokens (or mass).  A range of keys that is kept as a whole ends the
-// search; its last key is the cut.
+// The key at which the descending order reaches `target` tokens (or mass), looked for in bins r0 .. r1 of the first histogram, then,
+// if it is not there, in all of them: BINS finer ones of equal width (values near zero have many keys, neighbours of any
+// value few), then ranges of keys.  A range that is kept as a whole ends the search; its last key is the cut.
 __device__ __noinline__ lg::Cut descend(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, bool by_mass,
-                                           lg::u64 target) {
+                                        lg::u64 target, int r0, int r1) {
     using lg::Cut;
-    histogram(zs, slice, m, s, cl, [&](float z) { return linear_bin(m, z); });
-    find_crossing(s, by_mass, target, 0, 0);
-    if (s.bin < 0) return Cut{0xffffffffu, 0x7fffffff, 0, false};  // (only by count: fewer tokens than k)
-    unsigned int lo = s.bin == 0 ? down_key(m) : last_key(m, s.bin - 1) + 1, hi = last_key(m, s.bin);
-    for (int level = 0;; ++level) {  // (32 bits of key in steps of 10: four refinements at most)
-        const unsigned int above_count = s.w.above_count, count = s.w.bin_count;
-        const lg::u64 above_mass = s.w.above_mass, mass = s.w.bin_mass;
-        // a single token, or (by count) all of them: the range is kept as a whole
-        if (count == 1 || lo == hi || (!by_mass && above_count + count == target) || level == 4) {
-            Cut cut{hi, 0x7fffffff, above_mass + mass, true};
-            if (by_mass && count > 1) {
-                const lg::u64 each = mass / count, need = (target - above_mass + each - 1) / each;
-                if (need < count) cut.index = tie_cut(zs, slice, first, hi, (unsigned int)need, s, cl);
-            }
-            return cut;
-        }
-        const int bits = 32 - __clz(hi - lo), shift = bits > 10 ? bits - 10 : 0;
-        histogram(zs, slice, m, s, cl, [&](float z) {
-            const unsigned int k = down_key(z);
-            return k >= lo && k <= hi ? (int)((k - lo) >> shift) : -1;
-        });
-        find_crossing(s, by_mass, target, above_count, above_mass);
-        if (s.bin < 0) return Cut{hi, 0x7fffffff, above_mass + mass, true};
-        lo += (unsigned int)s.bin << shift;
-        const unsigned int end = lo + ((1u << shift) - 1);
-        hi = end < hi ? end : hi;
+    Cut cut{0xffffffffu, 0x7fffffff, 0, false};  // (by count: fewer tokens than k)
+    lg::u64 base_count = 0, base_mass = 0;
+    float start, scale;
+    const auto fine = [&](float z) {
+        const int b = linear_bin(m, z);
+        if (b < r0) return -1;
+        if (b > r1) return lg::BINS;
+        const float t = ((m - z) - start) * scale;
+        return t < (float)(lg::BINS - 1) ? max((int)t, 0) : lg::BINS - 1;
+    };
+    for (;; r0 = 0, r1 = lg::BINS - 1) {
+        start = (float)r0 / lg::BIN_SCALE, scale = lg::BIN_SCALE * (float)lg::BINS / (float)(r1 - r0 + 1);
+        histogram<true>(zs, slice, m, s, cl, base_count, base_mass, fine);
+        find_crossing(s, by_mass, target, (unsigned int)base_count, base_mass);
+        if (s.bin >= 0 || (r0 == 0 && r1 == lg::BINS - 1)) break;
+        __syncthreads();
     }
+    if (s.bin >= 0) {
+        // the last key of fine bins up to b: they rise with the key
+        const auto last = [&](int b) {
+            unsigned int lo = down_key(m), hi = down_key(-lg::FLOAT_MAX);
+            while (lo < hi) {
+                const unsigned int mid = lo + (hi - lo + 1) / 2;
+                if (fine(key_value(mid)) <= b) lo = mid;
+                else hi = mid - 1;
+            }
+            return lo;
+        };
+        unsigned int lo = fine(m) == s.bin ? down_key(m) : last(s.bin - 1) + 1, hi = last(s.bin);
+        for (int level = 0;; ++level) {  // (32 bits of key in steps of 10: four refinements at most)
+            const unsigned int above_count = s.w.above_count, count = s.w.bin_count;
+            const lg::u64 above_mass = s.w.above_mass, mass = s.w.bin_mass;
+            cut = Cut{hi, 0x7fffffff, above_mass + mass, true};
+            // a single token, or (by count) all of them: the range is kept as a whole
+            if (count == 1 || lo == hi || (!by_mass && above_count + count == target) || level == 4) {
+                if (by_mass && count > 1) {
+                    const lg::u64 each = mass / count, need = (target - above_mass + each - 1) / each;
+                    if (need < count) cut.index = tie_cut(zs, slice, first, hi, (unsigned int)need, s, cl);
+                }
+                break;
+            }
+            const int bits = 32 - __clz(hi - lo), shift = bits > 10 ? bits - 10 : 0;
+            histogram<false>(zs, slice, m, s, cl, base_count, base_mass, [&](float z) {
+                const unsigned int k = down_key(z);
+                return k >= lo && k <= hi ? (int)((k - lo) >> shift) : lg::BINS;
+            });
+            find_crossing(s, by_mass, target, above_count, above_mass);
+            if (s.bin < 0) break;
+            lo += (unsigned int)s.bin << shift;
+            const unsigned int end = lo + ((1u << shift) - 1);
+            hi = end < hi ? end : hi;
+        }
+    }
+    cl.sync();  // (the next list lies where the first CTA may still be reading)
+    return cut;
 }
 
 // ------------------------------ a window of bins around the cut, sorted
 // Which bins go on the list of the first CTA: from the first bin if what may be kept fits it, else a window around the cut; in
-// s.window_first, s.window_last (first > last: not even the cut's bin fits).  The cut's bin is known by count (k > 0), or
-// estimated: a bin's mass is taken as its count times e of its middle (1.6 % off at most), and two bins on either side allow
-// for that; the exact masses decide later.
-__device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, float want) {
+// s.window_first, s.window_last (first > last: not even the cut's bin fits).  `exact`: nothing beyond the cut's bin is needed.
+__device__ __forceinline__ void place_window(lg::Shared& s, int bin, bool exact) {
+    if (threadIdx.x == 0) {
+        const int wide = exact ? bin : min(bin + 2, lg::BINS - 1);
+        int first = 0, last = wide;
+        if (s.upto[wide] > lg::LIST) {
+            first = exact ? bin : max(bin - 2, 0);
+            auto tokens = [&] { return s.upto[last] - (first ? s.upto[first - 1] : 0); };
+            while (first <= last && tokens() > lg::LIST) {
+                if (last > bin) --last;
+                else ++first;
+            }
+        }
+        s.window_first = first, s.window_last = last;
+    }
+    __syncthreads();
+}
+// The cut's bin (s.bin) and the window.  The bin is known by count (k > 0), or
+// estimated: a bin's mass is taken as its count times e of its middle (1.6 % off at most).  Few heavy tokens make most of that
+// error, above the cut, so what the estimate of the whole row is off by (`all`: the row's mass) is taken as the error at the cut too (of 64 rows of
+// normal logits 4 missed the window without this); two bins on either side allow for the rest.  The exact masses decide later.
+__device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, float want, float all) {
     static_assert(lg::BINS == 2 * lg::THREADS, "two bins a thread");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = 2 * threadIdx.x;
     if (threadIdx.x == 0) s.bin = lg::BINS - 1;
@@ -475,33 +538,25 @@ __device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, flo
         }
         if (lane == 31) s.warp_est[warp] = q;
         __syncthreads();
-        for (int w = 0; w < warp; ++w) q += s.warp_est[w];
-        const bool before = q - q0 - q1 >= want;
-        // (rounding may let two neighbours claim the crossing, or none: the last bin then)
-        if (!before && q >= want) s.bin = q - q1 >= want ? b : b + 1;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int bin = s.bin, wide = k ? bin : min(bin + 2, lg::BINS - 1);
-        int first = 0, last = wide;
-        if (s.upto[wide] > lg::LIST) {
-            first = k ? bin : max(bin - 2, 0);
-            auto tokens = [&] { return s.upto[last] - (first ? s.upto[first - 1] : 0); };
-            while (first <= last && tokens() > lg::LIST) {
-                if (last > bin) --last;
-                else ++first;
-            }
+        float total = 0.0f;
+        for (int w = 0; w < lg::WARPS; ++w) {
+            if (w < warp) q += s.warp_est[w];
+            total += s.warp_est[w];
         }
-        s.window_first = first, s.window_last = last;
+        want += total - all;
+        const bool before = q - q0 - q1 >= want;
+        // (rounding may let two neighbours claim the crossing: the first of them, in every CTA; or none: the last bin then)
+        if (!before && q >= want) atomicMin(&s.bin, q - q1 >= want ? b : b + 1);
     }
     __syncthreads();
+    place_window(s, s.bin, k != 0);
 }
 
 // Every token of the window, no key beyond `limit`, to the first CTA's list; the masses (if asked for) of it and of what lies
 // above to every CTA.  `few`: so few tokens that each takes its own place, else a CTA takes places for all of its at once.  Ends
 // with a cluster barrier.
 template <int VEC>
-__device__ __forceinline__ void gather(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, int stage,
+__device__ __forceinline__ void gather(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, int turn,
                                        unsigned int limit, bool masses, bool few) {
     using lg::u64;
     const int w0 = s.window_first, w1 = s.window_last, C = cl.num_blocks(), rank = cl.block_rank();
@@ -510,7 +565,7 @@ __device__ __forceinline__ void gather(const float* zs, int slice, int first, fl
     if (!few) {
         for (int b = w0 + threadIdx.x; b <= w1; b += lg::THREADS) mine += s.count[b];
         mine = block_add(mine, s.warp_mass);
-        if (threadIdx.x == 0) s.list_base = mine ? atomicAdd(&head->list_n[stage], (unsigned int)mine) : 0, s.list_at = 0;
+        if (threadIdx.x == 0) s.list_base = mine ? atomicAdd(&head->list_n[turn], (unsigned int)mine) : 0, s.list_at = 0;
         __syncthreads();
     }
     u64 above = 0, listed = 0;
@@ -526,7 +581,7 @@ __device__ __forceinline__ void gather(const float* zs, int slice, int first, fl
             const unsigned int key = down_key(z);
             const bool in = key <= limit;
             if (in) listed += e;
-            const unsigned int at = few ? atomicAdd(&head->list_n[stage], 1u) : s.list_base + atomicAdd(&s.list_at, 1u);
+            const unsigned int at = few ? atomicAdd(&head->list_n[turn], 1u) : s.list_base + atomicAdd(&s.list_at, 1u);
             head->list[at] = in ? (u64)key << 32 | (unsigned int)(first + j) : ~0ull;
         });
     if (masses) {
@@ -534,7 +589,7 @@ __device__ __forceinline__ void gather(const float* zs, int slice, int first, fl
         listed = block_add(listed, s.warp_mass);
         if ((int)threadIdx.x < C) {
             lg::Shared* o = cl.map_shared_rank(&s, threadIdx.x);
-            o->mass_of[stage][0][rank] = above, o->mass_of[stage][1][rank] = listed;
+            o->mass_of[turn][0][rank] = above, o->mass_of[turn][1][rank] = listed;
         }
     }
     cl.sync();
@@ -725,25 +780,33 @@ __device__ __forceinline__ void finish(const float* zs, int slice, int first, fl
     int ones = 0;  // e = 1 is counted apart: a sure token's log-probability is all in the small terms
     if ((sums || !d.greedy) && m != -INFINITY)
         for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
+            float z[VEC], e[VEC], n[VEC];
+            bool in[VEC];
 #pragma unroll
             for (int h = 0; h < VEC; h += 4) {
                 const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
-                const float z[4] = {w.x, w.y, w.z, w.w};
-                const int v0 = first + j + h;
+                z[h] = w.x, z[h + 1] = w.y, z[h + 2] = w.z, z[h + 3] = w.w;
+            }
+            // the noise of what is kept, requested together (one by one each waits for its own: 64 rows, top-p FIXME us)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int v = first + j + i;
+                e[i] = fast_exp(z[i] - m);  // (0 of what is not there)
+                in[i] = !d.greedy && z[i] != -INFINITY && keep(z[i], v, e[i]);
+                n[i] = 1.0f;
+                if (in[i]) n[i] = q[v];
+            }
+#pragma unroll
+            for (int h = 0; h < VEC; h += 4) {
                 float part = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = fast_exp(z[i] - m);  // (0 of what is not there)
-                    if (sums) {
-                        if (e == 1.0f) ++ones;
-                        else part += e;
-                    }
-                    if (!d.greedy && z[i] != -INFINITY && keep(z[i], v0 + i, e)) {
-                        const float score = race_score(e, q[v0 + i]);
-                        if (score > best.score) best.score = score, best.index = v0 + i, best.z = z[i];  // (tokens come in order)
-                    }
+                for (int i = h; i < h + 4; ++i) {
+                    if (e[i] == 1.0f) ++ones;
+                    else part += e[i];
+                    const float score = race_score(e[i], n[i]);
+                    if (in[i] && score > best.score) best.score = score, best.index = first + j + i, best.z = z[i];  // (tokens come in order)
                 }
-                if (sums) best.sum += (double)part;
+                best.sum += (double)part;
             }
         }
     best.sum += (double)ones;
@@ -880,7 +943,7 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
     const int64_t row = blockIdx.x / C;
     const T* in = logits + row * ld;
     const int first = rank * slice - (int)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % VEC);
-    if (threadIdx.x < 2) s.list_n[threadIdx.x] = 0;
+    if (threadIdx.x < 4) s.list_n[threadIdx.x] = 0;
     for (int b = threadIdx.x; b < BINS; b += THREADS) s.count[b] = 0, s.owned[b] = 0;
     cluster_arrive_relaxed();  // this CTA runs: the others may write into its shared memory
     grid_dependency_wait();
@@ -944,16 +1007,20 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
 #pragma unroll 1
         for (int stage = by_k && (unsigned int)k < s.upto[BINS - 1] ? 0 : 1; stage < (by_p ? 2 : 1); ++stage) {
             if (stage == 1 && cut_k.found) target_p = share_of(share, (double)cut_k.mass);
-            choose_window(s, stage == 0 ? (unsigned int)k : 0u, (float)((double)target_p / MASS_UNIT));
-            const int w0 = s.window_first, w1 = s.window_last;
+            choose_window(s, stage == 0 ? (unsigned int)k : 0u, (float)((double)target_p / MASS_UNIT), (float)all);
+            // where the descent looks first if there is no list
+            int r0 = stage == 0 ? s.bin : max(s.bin - 2, 0), r1 = stage == 0 ? s.bin : min(s.bin + 2, BINS - 1);
             bool done = false;
-            if (w0 <= w1) {
+#pragma unroll 1
+            for (int turn = 2 * stage; turn < 2 * stage + 2 && !done; ++turn) {
+                const int w0 = s.window_first, w1 = s.window_last;
+                if (w0 > w1) break;
                 // (on a list that holds all that top-k keeps the first CTA finds the masses itself)
                 const bool masses = by_p && !(stage == 0 && w0 == 0);
                 const unsigned int tokens = s.upto[w1] - (w0 ? s.upto[w0 - 1] : 0);
-                gather<VEC>(zs, slice, first, m, s, cl, stage, cut_k.key, masses, tokens <= 128);
+                gather<VEC>(zs, slice, first, m, s, cl, turn, cut_k.key, masses, tokens <= 128);
                 u64 above = 0, listed = 0;
-                for (int c = 0; masses && c < C; ++c) above += s.mass_of[stage][0][c], listed += s.mass_of[stage][1][c];
+                for (int c = 0; masses && c < C; ++c) above += s.mass_of[turn][0][c], listed += s.mass_of[turn][1][c];
                 // (by count the window is right; by mass the exact one has to agree, or everything is on the list)
                 const bool right = stage == 0 || (above < target_p && above + listed >= target_p) || (w0 == 0 && w1 == BINS - 1);
                 if (right && w0 == 0 && rank) return;  // the first CTA has all that may be kept
@@ -1006,10 +1073,16 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
                     cl.sync();
                     (stage == 0 ? cut_k : cut_p) = s.cut[stage];
                     done = true;
+                } else {  // the cut lies in a bin before the window, or after it: the window beside it, once
+                    const bool before = above >= target_p;
+                    const int bin = before ? w0 - 1 : min(w1 + 1, BINS - 1);
+                    r0 = before ? max(bin - 3, 0) : bin, r1 = before ? bin : min(bin + 3, BINS - 1);
+                    __syncthreads();
+                    place_window(s, bin, false);
                 }
             }
             if (!done) {
-                const Cut cut = descend(zs, slice, first, m, s, cl, stage == 1, stage == 0 ? (u64)k : target_p);
+                const Cut cut = descend(zs, slice, first, m, s, cl, stage == 1, stage == 0 ? (u64)k : target_p, r0, r1);
                 (stage == 0 ? cut_k : cut_p) = cut;
             }
         }

@@ -269,6 +269,21 @@ def test_close_values_in_one_bin():
         assert int(hb.sample_tokens(tiny, noise, top_k=k)) == int(keep[(1 / noise[0, keep]).argmax()])
 
 
+@pytest.mark.parametrize("B", [2, 40])
+@pytest.mark.parametrize("dtype,width", [("fp32", 1e-3), ("fp32", 0.25), ("fp16", 0.25), ("bf16", 1.5), ("fp32", 6.0)])
+@pytest.mark.parametrize("k,p,mp", [(0, 0.9, 0.0), (0, 0.1, 0.0), (3000, 1.0, 0.0), (5000, 0.5, 0.0), (0, 0.6, 0.7)])
+def test_draw_of_flat_rows(B, dtype, width, k, p, mp):
+    """More tokens near the cut than can be sorted, around zero (where values have the most keys), a third of them masked."""
+    V = 40000
+    rng = np.random.default_rng(7)
+    z = rng.uniform(-0.5, 0.5, (B, V)) * width
+    z[rng.random((B, V)) < 1 / 3] = -np.inf
+    z = torch.from_numpy(z).to(DT[dtype]).cuda()
+    noise = noise_for(B, V, seed=11)
+    got, lp = hb.sample_tokens(z, noise, top_k=k, top_p=p, min_p=mp, return_logprobs=True)
+    check_draw(z, noise, got, lp, 1.0, k, p, mp)
+
+
 def test_next_token_is_what_tensor_code_draws():
     """``sample_next_token`` from one generator against the same steps in tensor code, the reference's order: temperature, top-k, top-p,
     a multinomial draw."""
