@@ -773,12 +773,16 @@ __device__ __forceinline__ void answer(const lg::Part& mine, bool greedy, lg::Sh
 
 // Sum of exponentials and the race over this CTA's tokens that `keep(key, token, e)` lets in, and the row's answer from the parts
 template <int VEC, typename F>
-__device__ __forceinline__ void finish(const float* zs, int slice, int first, float m, int top, const Draw& d, const float* q, bool sums,
-                                       lg::Shared& s, cg::cluster_group& cl, long long* token, float* logprob, F keep) {
+__device__ __noinline__ void finish(int slice, int first, float m, int top, bool greedy, const float* q, long long* token, float* logprob, F keep) {
     using lg::Part;
+    extern __shared__ __align__(16) unsigned char smem[];
+    lg::Shared& s = *reinterpret_cast<lg::Shared*>(smem);
+    const float* zs = reinterpret_cast<const float*>(smem + lg::FILTER_SHARED);
+    cg::cluster_group cl = cg::this_cluster();
+    const bool sums = logprob != nullptr;
     Part best{0.0, m, -1.0f, 0.0f, top, 0x7fffffff};
     int ones = 0;  // e = 1 is counted apart: a sure token's log-probability is all in the small terms
-    if ((sums || !d.greedy) && m != -INFINITY)
+    if ((sums || !greedy) && m != -INFINITY)
         for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
             float z[VEC], e[VEC], n[VEC];
             bool in[VEC];
@@ -787,14 +791,18 @@ __device__ __forceinline__ void finish(const float* zs, int slice, int first, fl
                 const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
                 z[h] = w.x, z[h + 1] = w.y, z[h + 2] = w.z, z[h + 3] = w.w;
             }
-            // the noise of what is kept, requested together (one by one each waits for its own: 64 rows, top-p FIXME us)
+            bool any = false;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const int v = first + j + i;
                 e[i] = fast_exp(z[i] - m);  // (0 of what is not there)
-                in[i] = !d.greedy && z[i] != -INFINITY && keep(z[i], v, e[i]);
-                n[i] = 1.0f;
-                if (in[i]) n[i] = q[v];
+                in[i] = !greedy && z[i] != -INFINITY && keep(z[i], first + j + i, e[i]);
+                n[i] = 1.0f, any |= in[i];
+            }
+            // the noise of what is kept, requested together: no load waits for a condition (of the others the first token's is read instead).
+            // 256 rows, top-k 5000: 152 -> 138 us, 64 rows 34.9 -> 36.8, one row 21.4 -> 20.8
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) n[i] = q[in[i] ? first + j + i : 0];
             }
 #pragma unroll
             for (int h = 0; h < VEC; h += 4) {
@@ -811,7 +819,7 @@ __device__ __forceinline__ void finish(const float* zs, int slice, int first, fl
         }
     best.sum += (double)ones;
     best = block_part(best, s);
-    answer(best, d.greedy, s, cl, token, logprob);
+    answer(best, greedy, s, cl, token, logprob);
 }
 
 // Rows without any filter: one pass over logits and noise, everything relative to the largest value that a thread has met so far
@@ -1089,10 +1097,10 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
     }
     const unsigned int key = cut_k.key < cut_p.key ? cut_k.key : cut_p.key;
     const float least = d.min_p > 0.0f ? d.min_p : 0.0f;
-    finish<VEC>(zs, slice, first, m, top, d, q, logprob != nullptr, s, cl, token + row, logprob ? logprob + row : nullptr,
-                [&](float z, int v, float e) {
+    finish<VEC>(slice, first, m, top, d.greedy, q, token + row, logprob ? logprob + row : nullptr,
+                [key, least, at_key = cut_p.key, from = cut_p.index](float z, int v, float e) {
                     const unsigned int kk = down_key(z);
-                    return kk <= key && e >= least && !(kk == cut_p.key && v >= cut_p.index);
+                    return kk <= key && e >= least && !(kk == at_key && v >= from);
                 });
 }
 
