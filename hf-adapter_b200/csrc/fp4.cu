@@ -138,7 +138,8 @@ __device__ __forceinline__ uint32_t encode_piece(const Piece<T>& piece, int ge, 
 }
 
 // `team` threads a row, P pieces of 16 elements a thread, read once and kept (P = 0: read again for the codes).  Rows beyond R
-// pad the last scale tile with zeros.  Bound by the memory: FIXME
+// pad the last scale tile with zeros.  Bound by the memory for many rows, where nvfp4 also waits for the row's maximum before its first code: 8192 x 4096
+// bf16 (67 MB in, 18 to 19 out) mxfp4 14.8 us = 5.7 TB/s, nvfp4 20.9 us = 4.1 TB/s; by the launch for few: 1 x 768 1.3 and 1.8 us, 64 x 4096 1.7 and 2.1.
 template <typename T, int FORMAT, int P>
 __global__ void __launch_bounds__(256) fp4_quant_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ packed,
                                                         uint8_t* __restrict__ scales, float* __restrict__ row_scale, int R, int K, int team) {
@@ -203,7 +204,8 @@ __global__ void __launch_bounds__(256) fp4_quant_kernel(const T* __restrict__ x,
     }
 }
 
-// 16 bytes of values a thread, four of them a turn; INDEX wide enough to count them
+// 16 bytes of values a thread, four of them a turn; INDEX wide enough to count them.  Bound by the memory: 8192 x 4096 to bf16 (85 MB) 16.2 us
+// (mxfp4) and 17.5 us (nvfp4) = 5.2 and 4.9 TB/s.
 template <typename T, int FORMAT, typename INDEX>
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t* __restrict__ packed, const uint8_t* __restrict__ scales,
                                                           const float* __restrict__ row_scale, T* __restrict__ out, INDEX total, int K) {
@@ -249,7 +251,8 @@ template <typename T, int FORMAT>
 static int quant(const void* x, int64_t ldx, uint8_t* packed, uint8_t* scales, float* row_scale, int rows, int K, cudaStream_t st) {
     const int ktiles = k_tiles(K, FORMAT);
     const int pieces = ktiles * SCALE_TILE_BLOCKS * block_of(FORMAT) / 16;
-    // Few rows: a piece a thread, for the shortest way.  Many rows: four, and several rows a CTA.  (FIXME)
+    // Few rows: a piece a thread, for the shortest way.  Many rows: four, and several rows a CTA.  us with one / four, nvfp4: 1 x 4096 2.1 / 3.2, 512 x 4096
+    // 3.4 / 3.8, 1024 x 4096 4.6 / 4.6 (mxfp4 3.0 / 3.4), 8192 x 4096 22.6 / 19.2, 8192 x 768 6.7 / 5.4; one row a CTA there 9.5.
     const int per = rows >= 2048 ? 4 : 1;
     int team = 32;
     while (team < 256 && team * per < pieces) team *= 2;

@@ -122,7 +122,9 @@ constexpr int tmem_cols(int format, int bn, bool deep) { return f4::pow2_cols(bn
 // in turn).  A lane is a channel: what a warp stores or reads for one token is 32 neighbouring channels, whole sectors.
 // The kernel before this one in the stream is the quantiser of the tokens: only their codes, scales and row factors wait for
 // it.  It has itself waited for everything earlier before it let this kernel start, so the weight, bias and residual are there.
-// (B200, nvfp4: 1 x 4096 -> 16384 streams 37.8 MB of weight in FIXME)
+// Bound by the weight's way from memory where there is much of it, else by the launch, the quantiser before it and the chain load, MMA, exchange, store.  us a
+// call, quantiser included, weights out of memory, nvfp4: 1 x 4096 -> 65536 (151 MB) 27.6 = 5.5 TB/s, 1 x 4096 -> 16384 (37.7 MB) 10.9, 1 x 4096 -> 4096
+// 6.1, 64 x 4096 -> 4096 8.6.
 template <int FORMAT, typename T, int BN, bool DEEP>
 __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(const __grid_constant__ Fp4Maps maps, const Fp4Args p) {
     using namespace fs;
@@ -306,6 +308,10 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
 // leader's commits arrive on empty[s] / acc_full[a] in both CTAs; the epilogue warps of both arrive on the leader's acc_empty[a].
 // Each CTA stages its own 128 token rows, half of the channels, the scales of its own rows and those of all channels
 // (each CTA's tensor memory needs them).  Eight epilogue warps, two a lane quarter, each with half of the columns.
+// A pair reads 64 KB a stage of 256 k for 512 cycles of MMA: bound by the way from L2 into shared memory (54 to 75 bytes a cycle and SM) and, in
+// long products, by the power cap.  Device us, quantiser included, fp16 out: 8192 x 4096 -> 16384 nvfp4 243 to 267 (1.1 TFLOP; the quantiser 20 of it: 4.9
+// PFLOP/s, three times the measured bf16 rate), mxfp4 232; 2048 x 4096 -> 16384 65.8; 777 x 2560 -> 10240 22.6 and 20.2 (160 tiles on 74 pairs: three
+// turns, the last one for 12).
 namespace fp {
 constexpr int BM = 128, PAIR_M = 256, EW = 8, THREADS = 64 + 32 * EW, STAGES = 5, A_BYTES = BM * f4::KSB, GROUP_M = 16;
 constexpr int b_bytes(int bn) { return bn / 2 * f4::KSB; }

@@ -2,7 +2,7 @@
 //
 // Rules (both kernels), in fp32, z the logit of token v, c how often v was generated, seen whether it occurs in the history at all:
 //   seen: z > 0 ? z / repetition : z * repetition;  then  z - frequency * c - presence * (c > 0) + bias[v];  not allowed: -inf.
-// Draw (sample_kernel), z / temperature, m the row's largest value, e = exp(z - m):
+// Draw (pick_kernel, filter_kernel), z / temperature, m the row's largest value, e = exp(z - m):
 //   top-k  keeps z >= the k-th largest (ties stay);
 //   top-p  keeps, in descending order (of equal values the lowest index first), every token with less than p of the mass of the
 //          top-k survivors before it; the first always;
@@ -29,6 +29,7 @@ constexpr int MAX_CLUSTER = 8;
 constexpr int BINS = 1024;           // of a histogram
 constexpr float BIN_SCALE = 32.0f;   // first histogram: m - z in steps of 1/32, the last bin takes the rest
 constexpr int LIST = 1024;           // tokens that the short way sorts
+constexpr unsigned int FEW = 32;     // of which sorting costs next to nothing
 constexpr float MASS_UNIT = 1099511627776.0f;  // 2^40
 constexpr float FLOAT_MAX = 3.402823466e38f;
 
@@ -52,7 +53,7 @@ struct Shared {
     u64 mass_of[4][2][MAX_CLUSTER];   // [list][of the tokens above the window, of those on the list]
     u64 warp_mass[WARPS];
     double warp_sum[WARPS];
-    Cut cut[2];
+    Cut cut;
     float max[MAX_CLUSTER], warp_max[WARPS], warp_est[WARPS];
     int top[MAX_CLUSTER], warp_top[WARPS];
     unsigned int warp_count[WARPS];
@@ -62,8 +63,7 @@ struct Shared {
     unsigned int upto[BINS];          // the cluster's, summed from bin 0
     unsigned int list_n[4];           // first CTA: places given out on a list: top-k's, its second try, top-p's, its second try
     unsigned int list_base, list_at;
-    int bin, window_first, window_last;
-    int place;
+    int bin, reach, window_first, window_last;  // reach: the last bin up to which there are no more than FEW tokens
     union {
         u64 list[LIST];  // first CTA: down_key << 32 | token
         struct {         // the descent
@@ -166,29 +166,52 @@ __device__ __forceinline__ void load_vector(const T* in, int v0, int V, const Ro
     }
 }
 
-// counts the history's tokens in [first, first + n) into words[0, n); ids outside the vocabulary fall outside every slice
+// counts the history's tokens in [first, first + n) into words[0, n), n a multiple of 4; ids outside the vocabulary fall outside every
+// slice.  Four ids a thread are on their way while the words are cleared, and while the four before them are counted.
 __device__ __forceinline__ void count_history(const rwkv7_logit_rules& r, int64_t row, int first, int n, unsigned int* words) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) words[i] = 0;
-    __syncthreads();
+    constexpr int AHEAD = 4;
     int len = r.lengths ? r.lengths[row] : r.history;
     len = len < r.history ? len : r.history;
-    const int prompt = r.prompt_lengths ? r.prompt_lengths[row] : 0;
-    for (int i = threadIdx.x; i < len; i += blockDim.x) {
-        const int64_t id = r.tokens_i64 ? static_cast<const int64_t*>(r.tokens)[row * r.tokens_ld + i]
-                                        : (int64_t) static_cast<const int32_t*>(r.tokens)[row * r.tokens_ld + i];
-        const int64_t at = id - first;
-        if (id >= 0 && at >= 0 && at < n) {
-            if (i >= prompt) atomicAdd(&words[at], 1u);
-            else atomicOr(&words[at], 0x80000000u);
+    const int prompt = r.prompt_lengths ? r.prompt_lengths[row] : 0, T = blockDim.x;
+    const auto* wide = static_cast<const int64_t*>(r.tokens) + row * r.tokens_ld;
+    const auto* narrow = static_cast<const int32_t*>(r.tokens) + row * r.tokens_ld;
+    int64_t id[AHEAD];
+    const auto request = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = i0 + u * T;
+            id[u] = i >= len ? -1 : r.tokens_i64 ? wide[i] : (int64_t)narrow[i];
         }
+    };
+    request(threadIdx.x);
+    for (int i = threadIdx.x * 4; i < n; i += T * 4) *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (int i0 = threadIdx.x; i0 < len; i0 += AHEAD * T) {
+        int at[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int64_t d = id[u] - first;
+            at[u] = id[u] >= 0 && d >= 0 && d < n ? (int)d : -1;
+        }
+        request(i0 + AHEAD * T);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (at[u] >= 0) {
+                if (i0 + u * T >= prompt) atomicAdd(&words[at[u]], 1u);
+                else atomicOr(&words[at[u]], 0x80000000u);
+            }
     }
     __syncthreads();
 }
 
 // ---------------------------------------------------------------- rules alone
-// grid (slices, rows); a row of any alignment is walked in 16-byte vectors that begin up to 16 bytes before it
+// grid (slices, rows); a row of any alignment is walked in 16-byte vectors that begin up to 16 bytes before it.  A slice's history is
+// counted by its own CTA, which reads the row's whole history for that (out of L2 after the first): no second launch, no counts in memory.
+// Bound by the launch and the chain history -> counts -> logits for a row or two, by issued instructions for many: device us, 65536 tokens fp16,
+// one row and 300 tokens of history 3.6, 64 rows, 4096 tokens, a bias and a mask 14.2 (19.7 MB in and out: 1.4 TB/s), 256 rows, 300 tokens
+// 26.7 (67 MB: 2.5 TB/s).
 template <typename T>
-__global__ void __launch_bounds__(256) process_logits_kernel(const T* logits, int64_t ld, const rwkv7_logit_rules rules, T* out,
+__global__ void __launch_bounds__(512) process_logits_kernel(const T* logits, int64_t ld, const rwkv7_logit_rules rules, T* out,
                                                              int64_t out_ld, int V, int slice) {
     extern __shared__ unsigned int words[];
     constexpr int VEC = 16 / sizeof(T);
@@ -198,6 +221,8 @@ __global__ void __launch_bounds__(256) process_logits_kernel(const T* logits, in
     const int mis = (int)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % VEC);  // elements before the row in its first vector
     const bool vec_out = (reinterpret_cast<uintptr_t>(o) / sizeof(T)) % VEC == (uintptr_t)mis;
     const int first = blockIdx.x * slice - mis;  // token of the slice's first place (may lie before the row)
+    grid_dependency_wait();
+    grid_launch_dependents();
     const Row r = row_rules(rules, row);
     if (r.history) count_history(rules, row, first, slice, words);
     for (int j = threadIdx.x * VEC; j < slice; j += blockDim.x * VEC) {
@@ -235,21 +260,6 @@ __device__ __forceinline__ lg::u64 fixed_mass(float e) { return __float2ull_rn(e
 __device__ __forceinline__ lg::u64 share_of(double share, double mass) {
     const double want = ceil(share * mass);
     return want < 1.0 ? 1ull : (lg::u64)want;
-}
-
-// A slice is walked in its own vectors of VEC places by the thread that loaded them; `f(place, z)` for every token that is there.
-template <int VEC, typename F>
-__device__ __forceinline__ void each_token(const float* zs, int slice, F f) {
-    for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
-#pragma unroll
-        for (int h = 0; h < VEC; h += 4) {
-            const float4 q = *reinterpret_cast<const float4*>(zs + j + h);
-            const float z[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (z[i] != -INFINITY) f(j + h + i, z[i]);
-        }
-    }
 }
 
 // log of a sum that is at least 1
@@ -496,19 +506,23 @@ __device__ __noinline__ lg::Cut descend(const float* zs, int slice, int first, f
 }
 
 // ------------------------------ a window of bins around the cut, sorted
-// Which bins go on the list of the first CTA: from the first bin if what may be kept fits it, else a window around the cut; in
-// s.window_first, s.window_last (first > last: not even the cut's bin fits).  `exact`: nothing beyond the cut's bin is needed.
-__device__ __forceinline__ void place_window(lg::Shared& s, int bin, bool exact) {
+// Which bins go on the list of the first CTA, in s.window_first, s.window_last (first > last: not even the cut's bin fits).
+// `exact`: the cut is in this bin, else it may be in the two on either side.  From the first bin if no more than `room` tokens may be
+// kept (and, as sorting so few costs the same, as many bins as hold FEW where the cut is not exact: where tokens are few they are heavy,
+// and a cut that is missed by one may be many bins away), else around the cut alone: what lies above is then weighed and raced in passing, not sorted.
+__device__ __forceinline__ void place_window(lg::Shared& s, int bin, bool exact, unsigned int room) {
     if (threadIdx.x == 0) {
         const int wide = exact ? bin : min(bin + 2, lg::BINS - 1);
         int first = 0, last = wide;
-        if (s.upto[wide] > lg::LIST) {
+        if (s.upto[wide] > room) {
             first = exact ? bin : max(bin - 2, 0);
             auto tokens = [&] { return s.upto[last] - (first ? s.upto[first - 1] : 0); };
             while (first <= last && tokens() > lg::LIST) {
                 if (last > bin) --last;
                 else ++first;
             }
+        } else if (!exact) {
+            last = max(wide, s.reach);
         }
         s.window_first = first, s.window_last = last;
     }
@@ -518,7 +532,7 @@ __device__ __forceinline__ void place_window(lg::Shared& s, int bin, bool exact)
 // estimated: a bin's mass is taken as its count times e of its middle (1.6 % off at most).  Few heavy tokens make most of that
 // error, above the cut, so what the estimate of the whole row is off by (`all`: the row's mass) is taken as the error at the cut too (of 64 rows of
 // normal logits 4 missed the window without this); two bins on either side allow for the rest.  The exact masses decide later.
-__device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, float want, float all) {
+__device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, float want, float all, unsigned int room) {
     static_assert(lg::BINS == 2 * lg::THREADS, "two bins a thread");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = 2 * threadIdx.x;
     if (threadIdx.x == 0) s.bin = lg::BINS - 1;
@@ -538,61 +552,20 @@ __device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, flo
         }
         if (lane == 31) s.warp_est[warp] = q;
         __syncthreads();
-        float total = 0.0f;
+        float total = 0.0f, upto = 0.0f;
         for (int w = 0; w < lg::WARPS; ++w) {
-            if (w < warp) q += s.warp_est[w];
+            if (w == warp) upto = total;
             total += s.warp_est[w];
         }
-        want += total - all;
-        const bool before = q - q0 - q1 >= want;
-        // (rounding may let two neighbours claim the crossing: the first of them, in every CTA; or none: the last bin then)
-        if (!before && q >= want) atomicMin(&s.bin, q - q1 >= want ? b : b + 1);
+        want = fmaxf(want + (total - all), 1e-30f);
+        // each thread's bins begin at the very number at which its neighbour's end, so that one of them has the crossing (where
+        // rounding makes it two, the first, in every CTA)
+        q += upto;
+        const float left = __shfl_up_sync(0xffffffffu, q, 1), before = lane ? left : upto;
+        if (before < want && q >= want) atomicMin(&s.bin, before + q0 >= want ? b : b + 1);
     }
     __syncthreads();
-    place_window(s, s.bin, k != 0);
-}
-
-// Every token of the window, no key beyond `limit`, to the first CTA's list; the masses (if asked for) of it and of what lies
-// above to every CTA.  `few`: so few tokens that each takes its own place, else a CTA takes places for all of its at once.  Ends
-// with a cluster barrier.
-template <int VEC>
-__device__ __forceinline__ void gather(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, int turn,
-                                       unsigned int limit, bool masses, bool few) {
-    using lg::u64;
-    const int w0 = s.window_first, w1 = s.window_last, C = cl.num_blocks(), rank = cl.block_rank();
-    lg::Shared* head = cl.map_shared_rank(&s, 0);
-    u64 mine = 0;  // (tokens of the window in this slice; some may lie beyond the limit)
-    if (!few) {
-        for (int b = w0 + threadIdx.x; b <= w1; b += lg::THREADS) mine += s.count[b];
-        mine = block_add(mine, s.warp_mass);
-        if (threadIdx.x == 0) s.list_base = mine ? atomicAdd(&head->list_n[turn], (unsigned int)mine) : 0, s.list_at = 0;
-        __syncthreads();
-    }
-    u64 above = 0, listed = 0;
-    if (few || mine || (masses && w0))
-        each_token<VEC>(zs, slice, [&](int j, float z) {
-            const int b = linear_bin(m, z);
-            if (b > w1) return;
-            const u64 e = masses ? fixed_mass(expf(z - m)) : 0;
-            if (b < w0) {
-                above += e;
-                return;
-            }
-            const unsigned int key = down_key(z);
-            const bool in = key <= limit;
-            if (in) listed += e;
-            const unsigned int at = few ? atomicAdd(&head->list_n[turn], 1u) : s.list_base + atomicAdd(&s.list_at, 1u);
-            head->list[at] = in ? (u64)key << 32 | (unsigned int)(first + j) : ~0ull;
-        });
-    if (masses) {
-        if (w0) above = block_add(above, s.warp_mass);
-        listed = block_add(listed, s.warp_mass);
-        if ((int)threadIdx.x < C) {
-            lg::Shared* o = cl.map_shared_rank(&s, threadIdx.x);
-            o->mass_of[turn][0][rank] = above, o->mass_of[turn][1][rank] = listed;
-        }
-    }
-    cl.sync();
+    place_window(s, s.bin, k != 0, room);
 }
 
 // list[0, n) ascending, n at most LIST; what pads it to a power of two is the largest key
@@ -680,6 +653,77 @@ __device__ __forceinline__ float race_score(float e, float q) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(q));
     return e * r;
+}
+
+// Every token of the window, no key beyond `limit`, to the first CTA's list; the masses (if asked for) of it and of what lies
+// above to every CTA, and with `race` the best score of what lies above (no e below `least`) to the first.  `few`: so few tokens that each takes
+// its own place, else a CTA takes places for all of its at once.  Ends with a cluster barrier.
+template <int VEC>
+__device__ __forceinline__ void gather(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, int turn,
+                                       unsigned int limit, bool masses, bool few, bool race, float least, const float* q) {
+    using lg::u64;
+    const int w0 = s.window_first, w1 = s.window_last, C = cl.num_blocks(), rank = cl.block_rank();
+    lg::Shared* head = cl.map_shared_rank(&s, 0);
+    u64 mine = 0;  // (tokens of the window in this slice; some may lie beyond the limit)
+    if (!few) {
+        for (int b = w0 + threadIdx.x; b <= w1; b += lg::THREADS) mine += s.count[b];
+        mine = block_add(mine, s.warp_mass);
+        if (threadIdx.x == 0) s.list_base = mine ? atomicAdd(&head->list_n[turn], (unsigned int)mine) : 0, s.list_at = 0;
+        __syncthreads();
+    }
+    u64 above = 0, listed = 0;
+    lg::Part best{0.0, m, -1.0f, 0.0f, 0, 0x7fffffff};
+    const auto list = [&](int v, float z) {
+        const unsigned int key = down_key(z);
+        const bool in = key <= limit;
+        if (in && masses) listed += fixed_mass(expf(z - m));
+        const unsigned int at = few ? atomicAdd(&head->list_n[turn], 1u) : s.list_base + atomicAdd(&s.list_at, 1u);
+        head->list[at] = in ? (u64)key << 32 | (unsigned int)v : ~0ull;
+    };
+    if (few || mine || (w0 && (masses || race)))
+        for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC)
+#pragma unroll
+            for (int h = 0; h < VEC; h += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
+                const float z[4] = {w.x, w.y, w.z, w.w};
+                const int v0 = first + j + h;
+                if (w0 == 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (z[i] != -INFINITY && linear_bin(m, z[i]) <= w1) list(v0 + i, z[i]);
+                    continue;
+                }
+                bool over[4], any = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int b = z[i] != -INFINITY ? linear_bin(m, z[i]) : lg::BINS;
+                    over[i] = b < w0, any |= over[i];
+                    if (b >= w0 && b <= w1) list(v0 + i, z[i]);
+                }
+                if (!any) continue;
+                float n[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) n[i] = race ? q[over[i] ? v0 + i : 0] : 1.0f;  // (requested together, as in finish())
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = over[i] ? expf(z[i] - m) : 0.0f, score = race_score(e, n[i]);
+                    if (masses) above += fixed_mass(e);
+                    if (over[i] && e >= least && score > best.score) best.score = score, best.index = v0 + i, best.z = z[i];
+                }
+            }
+    if (masses) {
+        if (w0) above = block_add(above, s.warp_mass);
+        listed = block_add(listed, s.warp_mass);
+        if ((int)threadIdx.x < C) {
+            lg::Shared* o = cl.map_shared_rank(&s, threadIdx.x);
+            o->mass_of[turn][0][rank] = above, o->mass_of[turn][1][rank] = listed;
+        }
+    }
+    if (race) {
+        best = block_part(best, s);
+        if (threadIdx.x == 0) head->part[rank] = best;
+    }
+    cl.sync();
 }
 
 // The draw of one row, and which of its filters are on
@@ -822,7 +866,10 @@ __device__ __noinline__ void finish(int slice, int first, float m, int top, bool
     answer(best, greedy, s, cl, token, logprob);
 }
 
-// Rows without any filter: one pass over logits and noise, everything relative to the largest value that a thread has met so far
+// Rows without any filter: one pass over logits and noise, everything relative to the largest value that a thread has met so far.
+// The cluster of a row meets once, at the end, to compare its parts.  Bound by the launch and that chain for few rows, by issued instructions (0.6 a
+// cycle and scheduler, 35 a warp for its 32 tokens) for many.  Device us, 65536 tokens fp16, greedy / drawn: one row 4.3 / 5.4, 64 rows 6.6 / 10.0, 256 rows
+// 19.1 / 29.4 (33.6 MB and 101 MB: 1.8 and 3.4 TB/s); fp32 logits, 256 rows 21.4 / 31.5 (4.3 TB/s).
 template <typename T, bool RULES>
 __global__ void __launch_bounds__(lg::THREADS, 2) pick_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
                                                               const rwkv7_draw_params draw, const float* __restrict__ noise, int64_t noise_ld,
@@ -936,7 +983,12 @@ __global__ void __launch_bounds__(lg::THREADS, 2) pick_kernel(const T* __restric
     answer(x, greedy, s, cl, token + row, sums ? logprob + row : nullptr);
 }
 
-// Rows with filters
+// Rows with filters.  The cuts are found by counts in 1024 bins of m - z (and by what the bins weigh, estimated), which single out a
+// window of some hundred tokens; those alone are sorted, by the first CTA, with exact masses.  A row is in shared memory from the first pass
+// on.  Some 20 steps that wait for one another (barriers of CTA and cluster, a sort) bound it, for many rows the same with two CTAs an SM.  Device us, 65536
+// tokens fp16 with log-probability, one row / 64 / 256 rows: top-k 50 15.2 / 23.1 / 80, and with top-p the same; top-p 0.9 where 24 tokens are
+// likely 16 / 24 / 84; top-p 0.9 of normal logits (2400 tokens kept) 24 / 39 / 138; min-p 8.7 / 15 / 54; a flat row, which no
+// window holds, 47 / 94 / 350.
 template <typename T, bool RULES>
 __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
                                                                 const rwkv7_draw_params draw, const float* __restrict__ noise, int64_t noise_ld,
@@ -966,6 +1018,7 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
     block_max_index(m, top, s);
     cluster_wait();
     row_max(m, top, s, cl);
+    const float least = d.min_p > 0.0f ? d.min_p : 0.0f;
     Cut cut_k{0xffffffffu, 0x7fffffff, 0, false}, cut_p{0xffffffffu, 0x7fffffff, 0, false};
     if ((by_k || by_p) && m != -INFINITY) {
         // counts by distance from the largest value; every CTA sums up the bins it owns and reads the others' from their owners
@@ -1005,9 +1058,11 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
                 if (lane >= o) c += t;
             }
             if (lane == 31) s.warp_count[warp] = c;
+            if (threadIdx.x == 0) s.reach = BINS - 1;
             __syncthreads();
             for (int w = 0; w < warp; ++w) c += s.warp_count[w];
             s.upto[b] = c - n.y, s.upto[b + 1] = c;
+            if (c - n.x - n.y <= FEW && c > FEW) s.reach = c - n.y > FEW ? b - 1 : b;
             __syncthreads();
         }
         const double share = d.p > 0.0f ? (double)d.p : 0.0;
@@ -1015,7 +1070,12 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
 #pragma unroll 1
         for (int stage = by_k && (unsigned int)k < s.upto[BINS - 1] ? 0 : 1; stage < (by_p ? 2 : 1); ++stage) {
             if (stage == 1 && cut_k.found) target_p = share_of(share, (double)cut_k.mass);
-            choose_window(s, stage == 0 ? (unsigned int)k : 0u, (float)((double)target_p / MASS_UNIT), (float)all);
+            // The last cut's list is short rather than whole: us of one row, top-k 500 / 900 with the whole list 20.2 / 23.4, around the cut 17.7 /
+            // 18.1 (64 rows 33.8 / 37.0, 28.4 / 29.9), equal up to 128 tokens.  For top-k before top-p it is whole where that is possible, which
+            // saves the second list: top-k 500 then top-p one row 19.8, two lists 26.7.
+            const bool last = stage == 1 || !by_p;
+            const unsigned int room = last ? 128 : LIST;
+            choose_window(s, stage == 0 ? (unsigned int)k : 0u, (float)((double)target_p / MASS_UNIT), (float)all, room);
             // where the descent looks first if there is no list
             int r0 = stage == 0 ? s.bin : max(s.bin - 2, 0), r1 = stage == 0 ? s.bin : min(s.bin + 2, BINS - 1);
             bool done = false;
@@ -1026,27 +1086,29 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
                 // (on a list that holds all that top-k keeps the first CTA finds the masses itself)
                 const bool masses = by_p && !(stage == 0 && w0 == 0);
                 const unsigned int tokens = s.upto[w1] - (w0 ? s.upto[w0 - 1] : 0);
-                gather<VEC>(zs, slice, first, m, s, cl, turn, cut_k.key, masses, tokens <= 128);
+                // with the last cut in the window all above is kept, and what is kept of the list the first CTA finds: no other pass is needed
+                const bool race = last && w0;
+                gather<VEC>(zs, slice, first, m, s, cl, turn, cut_k.key, masses, tokens <= 128, race, least, q);
                 u64 above = 0, listed = 0;
                 for (int c = 0; masses && c < C; ++c) above += s.mass_of[turn][0][c], listed += s.mass_of[turn][1][c];
                 // (by count the window is right; by mass the exact one has to agree, or everything is on the list)
                 const bool right = stage == 0 || (above < target_p && above + listed >= target_p) || (w0 == 0 && w1 == BINS - 1);
-                if (right && w0 == 0 && rank) return;  // the first CTA has all that may be kept
+                if (right && (w0 == 0 || last) && rank) return;
                 if (right && rank == 0) {
                     const int n = (int)(s.upto[w1] - (w0 ? s.upto[w0 - 1] : 0));
                     sort_list(s.list, n);
                     const unsigned int above_count = w0 ? s.upto[w0 - 1] : 0;
-                    const unsigned int last = stage == 0 ? (unsigned int)(s.list[k - (int)above_count - 1] >> 32) : cut_k.key;
-                    const int kept = cut_k.found || stage == 0 ? places_upto(s.list, n, last) : n;
+                    const unsigned int key_k = stage == 0 ? (unsigned int)(s.list[k - (int)above_count - 1] >> 32) : cut_k.key;
+                    const int kept = cut_k.found || stage == 0 ? places_upto(s.list, n, key_k) : n;
                     const Places o = weigh_list(s.list, kept, m, above, s);
-                    const int i0 = threadIdx.x * 2;
-                    if (w0 == 0) {
+                    if (w0 == 0 || last) {
+                        const int i0 = threadIdx.x * 2;
                         const u64 target = !by_p ? ~0ull : stage == 0 ? share_of(share, (double)o.total) : target_p;
                         Part best{0.0, m, -1.0f, 0.0f, top, 0x7fffffff};
                         u64 before = o.before;
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            if (i0 + i < kept && before < target && o.e[i] >= (d.min_p > 0.0f ? d.min_p : 0.0f)) {
+                            if (i0 + i < kept && before < target && o.e[i] >= least) {
                                 const int v = (int)(unsigned int)s.list[i0 + i];
                                 const float score = race_score(o.e[i], q[v]);
                                 if (better(score, v, best.score, best.index)) best.score = score, best.index = v, best.z = o.z[i];
@@ -1055,38 +1117,30 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
                         }
                         best = block_part(best, s);
                         if (threadIdx.x == 0) {
+                            for (int c = 0; race && c < C; ++c) {
+                                const Part& x = s.part[c];
+                                if (better(x.score, x.index, best.score, best.index)) best.score = x.score, best.index = x.index, best.z = x.z;
+                            }
                             const bool drawn = best.index != 0x7fffffff;  // (noise of NaN alone: the most likely token)
                             token[row] = drawn ? best.index : top;
                             if (logprob) logprob[row] = ((drawn ? best.z : m) - m) - log_sum(all);
                         }
                         return;
                     }
-                    // the cut to every CTA
-                    Cut cut{0, 0x7fffffff, o.total, true};
-                    if (stage == 0) {
-                        cut.key = (unsigned int)(s.list[kept - 1] >> 32);
-                    } else {
-                        u64 before = o.before;
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            if (i0 + i < kept && before < target_p && before + o.w[i] >= target_p) s.place = i0 + i;
-                            before += o.w[i];
-                        }
-                        __syncthreads();
-                        cut.key = (unsigned int)(s.list[s.place] >> 32), cut.index = (int)(unsigned int)s.list[s.place] + 1;
-                    }
-                    if ((int)threadIdx.x < C) cl.map_shared_rank(&s, threadIdx.x)->cut[stage] = cut;
+                    // top-k's cut to every CTA, for top-p
+                    if ((int)threadIdx.x < C)
+                        cl.map_shared_rank(&s, threadIdx.x)->cut = Cut{(unsigned int)(s.list[kept - 1] >> 32), 0x7fffffff, o.total, true};
                 }
                 if (right) {
                     cl.sync();
-                    (stage == 0 ? cut_k : cut_p) = s.cut[stage];
+                    cut_k = s.cut;
                     done = true;
                 } else {  // the cut lies in a bin before the window, or after it: the window beside it, once
                     const bool before = above >= target_p;
                     const int bin = before ? w0 - 1 : min(w1 + 1, BINS - 1);
                     r0 = before ? max(bin - 3, 0) : bin, r1 = before ? bin : min(bin + 3, BINS - 1);
                     __syncthreads();
-                    place_window(s, bin, false);
+                    place_window(s, bin, false, room);
                 }
             }
             if (!done) {
@@ -1096,7 +1150,6 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
         }
     }
     const unsigned int key = cut_k.key < cut_p.key ? cut_k.key : cut_p.key;
-    const float least = d.min_p > 0.0f ? d.min_p : 0.0f;
     finish<VEC>(slice, first, m, top, d.greedy, q, token + row, logprob ? logprob + row : nullptr,
                 [key, least, at_key = cut_p.key, from = cut_p.index](float z, int v, float e) {
                     const unsigned int kk = down_key(z);
@@ -1123,14 +1176,23 @@ extern "C" int rwkv7_process_logits(const void* logits, int64_t ld, const rwkv7_
     RWKV7_REQUIRE(ld >= V && out_ld >= V, RWKV7_ERR_INVALID, "process_logits: a row stride is shorter than a row");
     RWKV7_REQUIRE(V <= (1 << 30), RWKV7_ERR_UNSUPPORTED, "process_logits: at most 2^30 tokens (got %d)", V);
     if (int e = check_rules("process_logits", rules)) return e;
-    const int slice = 8192;
+    // Tokens a CTA, a power of two made even over the row: few, so that a row or two spread over the GPU, more where the CTAs are
+    // many all the same and every one of them reads its row's history.  us, 65536 tokens, 1024 / 2048 / 4096 / 8192 a CTA (of 512 threads the last): one
+    // row, 300 of history 3.3 / 3.8 / 4.9 / 6.0; 16 rows, 1000 7.0 / 6.2 / 6.6 / 7.4; 64 rows, 512 16.9 / 13.1 / 12.2 / 12.4; 64
+    // rows, 4096 33.7 / 22.6 / 18.2 / 15.2; 256 rows, 300 53 / 34 / 26.7 / 28.5.
+    const int most = rules->tokens && rules->history > 1024 ? 8192 : 4096;
+    int slice = 1024;
+    while (slice < most && ((int64_t)V + slice - 1) / slice * B > 512) slice *= 2;
+    const int threads = slice < 8192 ? 256 : 512, slices = (V + slice - 1) / slice, places = V + 16 / (int)dtype_size(dtype) - 1;
+    slice = ((places + slices - 1) / slices + 7) / 8 * 8;
     const size_t smem = rules->tokens ? slice * 4 : 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaSuccess;
     RWKV7_DISPATCH_DTYPE(dtype, T, {
-        const int vec = 16 / sizeof(T);
-        process_logits_kernel<T><<<dim3((V + vec - 1 + slice - 1) / slice, B), 256, smem, st>>>(static_cast<const T*>(logits), ld, *rules,
-                                                                                                static_cast<T*>(out), out_ld, V, slice);
+        e = launch_programmatic(process_logits_kernel<T>, dim3(slices, B), dim3(threads), smem, st, static_cast<const T*>(logits), ld, *rules,
+                                static_cast<T*>(out), out_ld, V, slice);
     });
+    RWKV7_REQUIRE(e == cudaSuccess, RWKV7_ERR_CUDA, "process_logits: %s", cudaGetErrorString(e));
     return check_launch("process_logits_kernel");
 }
 
@@ -1180,5 +1242,5 @@ extern "C" int rwkv7_sample_tokens(const void* logits, int64_t ld, const rwkv7_l
         cfg.numAttrs = programmatic_launch_ok(st) ? 2 : 1;
         cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(logits), ld, *rules, *draw, noise, noise_ld, token, logprob, V, (int)slice);
     });
-    return check_launch("sample_kernel");
+    return check_launch(filters ? "filter_kernel" : "pick_kernel");
 }
