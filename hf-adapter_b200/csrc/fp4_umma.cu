@@ -668,7 +668,10 @@ static int dispatch_fp4(const void* w, const void* ws, const void* xq, const voi
         const int64_t stream = 20 + (tiles + kSMs - 1) / kSMs * ((splits > 1 ? 58 : 42) + stages / splits * 25 / 10);
         if (stream <= pair) return launch_stream<FORMAT, T, 128, true>(w, ws, xq, xs, a, st);
     }
-    if (waves(128) * 400 <= waves(256) * 600) return launch_pair<FORMAT, T, 128>(w, ws, xq, xs, a, st);
+    // a tile of half the channels takes two thirds of the time at best (its tokens are read as often, the way into shared memory bounds both) but
+    // leaves fewer pairs idle; us of 128 / 256 channels: 512 x 4096 -> 4096 (one turn either way) 12.4 / 13.8, 512 x 16384 -> 4096 27.9 / 32.1, 1536 x 16384 ->
+    // 4096 (three turns, two) 71.6 / 66.8, 1024 x 4096 -> 4096 (two, one) 18.1 / 15.9, 2048 x 4096 -> 16384 (14, 7) 78.3 / 64.9
+    if (waves(128) * 2 < waves(256) * 3) return launch_pair<FORMAT, T, 128>(w, ws, xq, xs, a, st);
     return launch_pair<FORMAT, T, 256>(w, ws, xq, xs, a, st);
 }
 
