@@ -262,6 +262,21 @@ __device__ __forceinline__ lg::u64 share_of(double share, double mass) {
     return want < 1.0 ? 1ull : (lg::u64)want;
 }
 
+// A slice is walked in its own vectors of VEC places by the thread that loaded them; `f(place, z)` for every token that is there.
+template <int VEC, typename F>
+__device__ __forceinline__ void each_token(const float* zs, int slice, F f) {
+    for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
+#pragma unroll
+        for (int h = 0; h < VEC; h += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(zs + j + h);
+            const float z[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (z[i] != -INFINITY) f(j + h + i, z[i]);
+        }
+    }
+}
+
 // log of a sum that is at least 1
 __device__ __forceinline__ float log_sum(double sum) { return log1pf((float)(sum - 1.0)); }
 
@@ -655,12 +670,45 @@ __device__ __forceinline__ float race_score(float e, float q) {
     return e * r;
 }
 
+// The best score of what lies above the window (no e below `least`) in this CTA's slice, to the first CTA.  A function of its own: inlined
+// it costs rows that do not need it half a microsecond of 16.
+template <int VEC>
+__device__ __noinline__ void race_above(int slice, int first, float m, float least, const float* q) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    lg::Shared& s = *reinterpret_cast<lg::Shared*>(smem);
+    const float* zs = reinterpret_cast<const float*>(smem + lg::FILTER_SHARED);
+    cg::cluster_group cl = cg::this_cluster();
+    const float edge = (float)s.window_first;  // linear_bin() below it
+    lg::Part best{0.0, m, -1.0f, 0.0f, 0, 0x7fffffff};
+    for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC) {
+        float z[VEC], n[VEC];
+        bool over[VEC], any = false;
+#pragma unroll
+        for (int h = 0; h < VEC; h += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
+            z[h] = w.x, z[h + 1] = w.y, z[h + 2] = w.z, z[h + 3] = w.w;
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) over[i] = (m - z[i]) * lg::BIN_SCALE < edge, any |= over[i];
+        if (!any) continue;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) n[i] = q[over[i] ? first + j + i : 0];  // (requested together, as in finish())
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float e = fast_exp(z[i] - m), score = race_score(e, n[i]);
+            if (over[i] && e >= least && score > best.score) best.score = score, best.index = first + j + i, best.z = z[i];
+        }
+    }
+    best = block_part(best, s);
+    if (threadIdx.x == 0) cl.map_shared_rank(&s, 0)->part[cl.block_rank()] = best;
+}
+
 // Every token of the window, no key beyond `limit`, to the first CTA's list; the masses (if asked for) of it and of what lies
-// above to every CTA, and with `race` the best score of what lies above (no e below `least`) to the first.  `few`: so few tokens that each takes
-// its own place, else a CTA takes places for all of its at once.  Ends with a cluster barrier.
+// above to every CTA.  `few`: so few tokens that each takes its own place, else a CTA takes places for all of its at once.  Ends
+// with a cluster barrier.
 template <int VEC>
 __device__ __forceinline__ void gather(const float* zs, int slice, int first, float m, lg::Shared& s, cg::cluster_group& cl, int turn,
-                                       unsigned int limit, bool masses, bool few, bool race, float least, const float* q) {
+                                       unsigned int limit, bool masses, bool few) {
     using lg::u64;
     const int w0 = s.window_first, w1 = s.window_last, C = cl.num_blocks(), rank = cl.block_rank();
     lg::Shared* head = cl.map_shared_rank(&s, 0);
@@ -672,45 +720,21 @@ __device__ __forceinline__ void gather(const float* zs, int slice, int first, fl
         __syncthreads();
     }
     u64 above = 0, listed = 0;
-    lg::Part best{0.0, m, -1.0f, 0.0f, 0, 0x7fffffff};
-    const auto list = [&](int v, float z) {
-        const unsigned int key = down_key(z);
-        const bool in = key <= limit;
-        if (in && masses) listed += fixed_mass(expf(z - m));
-        const unsigned int at = few ? atomicAdd(&head->list_n[turn], 1u) : s.list_base + atomicAdd(&s.list_at, 1u);
-        head->list[at] = in ? (u64)key << 32 | (unsigned int)v : ~0ull;
-    };
-    if (few || mine || (w0 && (masses || race)))
-        for (int j = threadIdx.x * VEC; j < slice; j += lg::THREADS * VEC)
-#pragma unroll
-            for (int h = 0; h < VEC; h += 4) {
-                const float4 w = *reinterpret_cast<const float4*>(zs + j + h);
-                const float z[4] = {w.x, w.y, w.z, w.w};
-                const int v0 = first + j + h;
-                if (w0 == 0) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (z[i] != -INFINITY && linear_bin(m, z[i]) <= w1) list(v0 + i, z[i]);
-                    continue;
-                }
-                bool over[4], any = false;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int b = z[i] != -INFINITY ? linear_bin(m, z[i]) : lg::BINS;
-                    over[i] = b < w0, any |= over[i];
-                    if (b >= w0 && b <= w1) list(v0 + i, z[i]);
-                }
-                if (!any) continue;
-                float n[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) n[i] = race ? q[over[i] ? v0 + i : 0] : 1.0f;  // (requested together, as in finish())
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = over[i] ? expf(z[i] - m) : 0.0f, score = race_score(e, n[i]);
-                    if (masses) above += fixed_mass(e);
-                    if (over[i] && e >= least && score > best.score) best.score = score, best.index = v0 + i, best.z = z[i];
-                }
+    if (few || mine || (masses && w0))
+        each_token<VEC>(zs, slice, [&](int j, float z) {
+            const int b = linear_bin(m, z);
+            if (b > w1) return;
+            const u64 e = masses ? fixed_mass(expf(z - m)) : 0;
+            if (b < w0) {
+                above += e;
+                return;
             }
+            const unsigned int key = down_key(z);
+            const bool in = key <= limit;
+            if (in) listed += e;
+            const unsigned int at = few ? atomicAdd(&head->list_n[turn], 1u) : s.list_base + atomicAdd(&s.list_at, 1u);
+            head->list[at] = in ? (u64)key << 32 | (unsigned int)(first + j) : ~0ull;
+        });
     if (masses) {
         if (w0) above = block_add(above, s.warp_mass);
         listed = block_add(listed, s.warp_mass);
@@ -718,10 +742,6 @@ __device__ __forceinline__ void gather(const float* zs, int slice, int first, fl
             lg::Shared* o = cl.map_shared_rank(&s, threadIdx.x);
             o->mass_of[turn][0][rank] = above, o->mass_of[turn][1][rank] = listed;
         }
-    }
-    if (race) {
-        best = block_part(best, s);
-        if (threadIdx.x == 0) head->part[rank] = best;
     }
     cl.sync();
 }
@@ -986,8 +1006,8 @@ __global__ void __launch_bounds__(lg::THREADS, 2) pick_kernel(const T* __restric
 // Rows with filters.  The cuts are found by counts in 1024 bins of m - z (and by what the bins weigh, estimated), which single out a
 // window of some hundred tokens; those alone are sorted, by the first CTA, with exact masses.  A row is in shared memory from the first pass
 // on.  Some 20 steps that wait for one another (barriers of CTA and cluster, a sort) bound it, for many rows the same with two CTAs an SM.  Device us, 65536
-// tokens fp16 with log-probability, one row / 64 / 256 rows: top-k 50 15.2 / 23.1 / 80, and with top-p the same; top-p 0.9 where 24 tokens are
-// likely 16 / 24 / 84; top-p 0.9 of normal logits (2400 tokens kept) 24 / 39 / 138; min-p 8.7 / 15 / 54; a flat row, which no
+// tokens fp16 with log-probability, one row / 64 / 256 rows: top-k 50 15.5 / 23.3 / 80, and with top-p the same; top-p 0.9 where 24 tokens are
+// likely 15.7 / 23.5 / 82; top-p 0.9 of normal logits (2400 tokens kept) 25 / 38 / 135; min-p 8.7 / 15 / 54; a flat row, which no
 // window holds, 47 / 94 / 350.
 template <typename T, bool RULES>
 __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
@@ -1088,7 +1108,8 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
                 const unsigned int tokens = s.upto[w1] - (w0 ? s.upto[w0 - 1] : 0);
                 // with the last cut in the window all above is kept, and what is kept of the list the first CTA finds: no other pass is needed
                 const bool race = last && w0;
-                gather<VEC>(zs, slice, first, m, s, cl, turn, cut_k.key, masses, tokens <= 128, race, least, q);
+                if (race) race_above<VEC>(slice, first, m, least, q);
+                gather<VEC>(zs, slice, first, m, s, cl, turn, cut_k.key, masses, tokens <= 128);
                 u64 above = 0, listed = 0;
                 for (int c = 0; masses && c < C; ++c) above += s.mass_of[turn][0][c], listed += s.mass_of[turn][1][c];
                 // (by count the window is right; by mass the exact one has to agree, or everything is on the list)
@@ -1164,6 +1185,7 @@ using namespace rwkv7;
 static int check_rules(const char* what, const rwkv7_logit_rules* r) {
     RWKV7_REQUIRE(r != nullptr, RWKV7_ERR_INVALID, "%s: null rules", what);
     RWKV7_REQUIRE(r->history >= 0, RWKV7_ERR_INVALID, "%s: negative history", what);
+    RWKV7_REQUIRE(r->history <= (1 << 30), RWKV7_ERR_UNSUPPORTED, "%s: at most 2^30 tokens of history (got %d)", what, r->history);
     RWKV7_REQUIRE(r->tokens == nullptr || r->tokens_ld >= r->history, RWKV7_ERR_INVALID, "%s: the history's stride is shorter than a row", what);
     return RWKV7_OK;
 }
