@@ -13,7 +13,7 @@
 // 256 x 256 or 256 x 128, persistent.  All waits are bounded (umma.cuh).
 #include <cooperative_groups.h>
 
-#include "fp4.cuh"
+#include "fp4_encode.cuh"
 #include "umma.cuh"
 
 namespace cg = cooperative_groups;
@@ -34,6 +34,8 @@ constexpr int pow2_cols(int need) {
 struct Fp4Args {
     const float *wg, *xg;  // row factors (nvfp4; NULL = 1)
     const void *bias, *residual;
+    const void* x;  // FUSED: the tokens, not quantised yet, ldx elements apart
+    int64_t ldx;
     void* y;
     int M, N, K;
     int relu2;
@@ -107,42 +109,102 @@ __device__ __forceinline__ void issue_stage(uint32_t d, uint64_t da, uint64_t db
 namespace fs {
 constexpr int BM = 128, EW = 8, THREADS = 64 + 32 * EW, A_BYTES = BM * f4::KSB, MAX_SPLITS = 8;
 constexpr int tokens_at_once(int bn) { return bn >= 64 ? 16 : 8; }  // of an epilogue warp
-constexpr int stage_bytes(int format, int bn) { return A_BYTES + bn * f4::KSB + 2 * f4::sf_bytes(format); }
+constexpr int FUSED_STAGES = 16;  // of tokens, which stay, where the kernel quantises them itself
+constexpr int ring_bytes(int format) { return A_BYTES + f4::sf_bytes(format); }                    // a stage of the weight
+constexpr int token_bytes(int format, int bn) { return bn * f4::KSB + f4::sf_bytes(format); }      // and one of tokens
 // DEEP: as many stages as fit, for grids of at most a CTA an SM; else room for two CTAs an SM where the tile is narrow
 constexpr int stages(int bn, bool deep) { return bn == 16 ? (deep ? 8 : 4) : bn == 32 ? (deep ? 8 : 3) : bn == 64 ? 6 : 4; }
 constexpr int q_bytes(int bn) { return bn * BM * 4; }  // partial sums of a tile
-constexpr int smem_bytes(int format, int bn, bool deep) {
-    return stages(bn, deep) * stage_bytes(format, bn) + q_bytes(bn) + f4::BAR_BYTES + bn * 4 + 1024;
+constexpr int smem_bytes(int format, int bn, bool deep, bool fused) {
+    return stages(bn, deep) * ring_bytes(format) + (fused ? FUSED_STAGES : stages(bn, deep)) * token_bytes(format, bn) + q_bytes(bn) + f4::BAR_BYTES +
+           bn * 4 + 1024;
 }
 constexpr int sf_cols(int format) { return f4::tiles_per_stage(format) * 8; }
 constexpr int tmem_cols(int format, int bn, bool deep) { return f4::pow2_cols(bn + stages(bn, deep) * sf_cols(format)); }
 }  // namespace fs
 
+// FUSED: the epilogue's threads make the tokens' operand themselves, codes in the 128-byte swizzle and scale tiles as the quantiser would
+// write them, for the K range of this CTA (stages kb0 .. kb0 + nk; nvfp4 needs the largest magnitude of whole rows for it).  `team` threads a row, 32 at
+// least; what lies beyond K is zero.  red: 8 floats.
+template <int FORMAT, typename T>
+__device__ __forceinline__ void quantise_tokens(const T* x, int64_t ldx, int M, int K, int kb0, int nk, unsigned char* codes, unsigned char* scales,
+                                                float* factor, float* red) {
+    constexpr int SF = f4::sf_bytes(FORMAT), THREADS = 32 * fs::EW, BN = 16;
+    const int tid = threadIdx.x - 64, lane = tid & 31;
+    int team = THREADS;
+    while (team > 32 && THREADS / team < M) team /= 2;
+    const int at = tid % team, pieces = K / 16;
+    for (int r0 = 0; r0 < M; r0 += THREADS / team) {
+        const int row = r0 + tid / team;
+        const bool live = row < M;
+        const T* xr = x + (live ? row : 0) * ldx;
+        int ge = 127;
+        if constexpr (FORMAT == fp4::NV) {
+            float m = 0.0f;
+#pragma unroll 4
+            for (int p = at; p < pieces; p += team) m = fmaxf(m, finite_amax(load_piece<T>(xr + 16 * p)));
+            m = group_max<32>(m);
+            if (team > 32) {
+                asm volatile("bar.sync 1, 256;" ::: "memory");  // (the last rows' maxima have been read)
+                if (lane == 0) red[tid >> 5] = m;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                for (int w = tid / team * (team / 32), n = team / 32; n > 0; ++w, --n) m = fmaxf(m, red[w]);
+            }
+            const int e = max(__float_as_int(m) >> 23, 1);
+            ge = m > 0.0f ? max(e - 10, 1) : 127;
+            if (at == 0 && live) factor[row] = __int_as_float(ge << 23);
+        } else if (at == 0 && live) {
+            factor[row] = 1.0f;
+        }
+#pragma unroll 2
+        for (int i0 = at - lane; i0 < 16 * nk; i0 += team) {  // (whole warps)
+            const int i = i0 + lane, p = 16 * kb0 + i;
+            Piece<T> piece{};
+            if (p < pieces) piece = load_piece<T>(xr + 16 * p);
+            uint2 c;
+            const uint32_t byte = encode_piece<T, FORMAT>(piece, ge, c);
+            if (live && i < 16 * nk) {
+                const int stage = i >> 4, j = i & 15;  // a piece: 8 bytes of the row's 128
+                *reinterpret_cast<uint2*>(codes + stage * (BN * f4::KSB) + row * f4::KSB + (((j >> 1) ^ (row & 7)) << 4) + (j & 1) * 8) = c;
+                const int block = FORMAT == fp4::NV ? j : j >> 1;
+                if (FORMAT == fp4::NV || !(j & 1))
+                    scales[stage * SF + (block >> 2) * fp4::SCALE_TILE_BYTES + row * 16 + (block & 3)] = (unsigned char)(p < pieces ? byte : 0);
+            }
+        }
+    }
+    fence_proxy_async_smem();
+}
+
 // grid (channel tiles, token tiles, splits); warp 0 = producer, warp 1 = MMA, warps 2..9 = epilogue (two a lane quarter,
 // in turn).  A lane is a channel: what a warp stores or reads for one token is 32 neighbouring channels, whole sectors.
 // The kernel before this one in the stream is the quantiser of the tokens: only their codes, scales and row factors wait for
 // it.  It has itself waited for everything earlier before it let this kernel start, so the weight, bias and residual are there.
-// Bound by the weight's way from memory where there is much of it, else by the launch, the quantiser before it and the chain load, MMA, exchange, store.  us a
-// call, quantiser included, weights out of memory, nvfp4: 1 x 4096 -> 65536 (151 MB) 27.6 = 5.5 TB/s, 1 x 4096 -> 16384 (37.7 MB) 10.9, 1 x 4096 -> 4096
-// 6.1, 64 x 4096 -> 4096 8.6.
-template <int FORMAT, typename T, int BN, bool DEEP>
+// FUSED: there is no quantiser, the tokens are quantised here under the first loads of the weight (quantise_tokens); everything waits for the
+// kernel before.
+// Bound by the weight's way from memory where there is much of it, else by the launch, the quantiser and the chain load, MMA, exchange, store.  us a
+// call, weights out of memory, nvfp4: 1 x 4096 -> 65536 (151 MB) 27.6 = 5.5 TB/s, 1 x 4096 -> 16384 (37.7 MB) 9.6, 1 x 4096 -> 4096
+// 6.6, 64 x 4096 -> 4096 8.6.
+template <int FORMAT, typename T, int BN, bool DEEP, bool FUSED>
 __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(const __grid_constant__ Fp4Maps maps, const Fp4Args p) {
     using namespace fs;
-    constexpr int STAGES = stages(BN, DEEP), SF = f4::sf_bytes(FORMAT), TMEM_COLS = tmem_cols(FORMAT, BN, DEEP), STAGE_BYTES = stage_bytes(FORMAT, BN);
+    constexpr int STAGES = stages(BN, DEEP), SF = f4::sf_bytes(FORMAT), TMEM_COLS = tmem_cols(FORMAT, BN, DEEP);
+    constexpr int TOKEN_STAGES = FUSED ? FUSED_STAGES : STAGES, STAGE_BYTES = ring_bytes(FORMAT) + (FUSED ? 0 : token_bytes(FORMAT, BN));
     constexpr int TB = tokens_at_once(BN);
     static_assert(BN + STAGES * sf_cols(FORMAT) <= TMEM_COLS && TMEM_COLS <= 512, "tensor memory");
-    static_assert(smem_bytes(FORMAT, BN, DEEP) <= (DEEP ? 227 : 113) * 1024, "shared memory");
+    static_assert(smem_bytes(FORMAT, BN, DEEP, FUSED) <= (DEEP ? 227 : 113) * 1024, "shared memory");
     static_assert(DEEP || TMEM_COLS <= 256, "tensor memory for two");
     extern __shared__ unsigned char smem_unaligned[];
     unsigned char* sm = smem_unaligned + ((1024u - (smem_u32(smem_unaligned) & 1023u)) & 1023u);
-    // [A of all stages][B of all stages][scales of all stages][partial sums: split, token, channel][barriers][row factors]
+    // [A of all stages][B of all stages][scales of A][scales of B][partial sums: split, token, channel][barriers][row factors]
     unsigned char* sm_b = sm + STAGES * A_BYTES;
-    unsigned char* sm_s = sm_b + STAGES * BN * f4::KSB;
-    float* Q = reinterpret_cast<float*>(sm + STAGES * STAGE_BYTES);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm + STAGES * STAGE_BYTES + q_bytes(BN));
+    unsigned char* sm_s = sm_b + TOKEN_STAGES * BN * f4::KSB;
+    unsigned char* sm_t = sm_s + STAGES * SF;
+    float* Q = reinterpret_cast<float*>(sm_t + TOKEN_STAGES * SF);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm_t + TOKEN_STAGES * SF + q_bytes(BN));
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+    uint64_t* tokens_full = acc_full + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tokens_full + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* s_xg = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(full) + f4::BAR_BYTES);
     const AbortCtx actx{abort_flag, p.error};
@@ -156,15 +218,20 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
     if (tid == 0) {
         for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
         mbar_init(acc_full, 1);
+        mbar_init(tokens_full, 1);
         *abort_flag = 0;
         mbar_fence_init();
-        // the weight does not depend on the kernel before this one: what the ring holds is requested under it
-        for (int i = 0; i < STAGES && i < nk; ++i) {
-            mbar_expect_tx(&full[i], STAGE_BYTES);
-            tma_load_2d(sm + i * A_BYTES, &maps.w, &full[i], (kb0 + i) * f4::KSB, n0);
-            tma_load_2d(sm_s + i * 2 * SF, &maps.ws, &full[i], (kb0 + i) * (SF / 8), blockIdx.x);
+        if constexpr (FUSED) {
+            tma_prefetch_desc(&maps.w), tma_prefetch_desc(&maps.ws);
+        } else {
+            // the weight does not depend on the kernel before this one: what the ring holds is requested under it
+            for (int i = 0; i < STAGES && i < nk; ++i) {
+                mbar_expect_tx(&full[i], STAGE_BYTES);
+                tma_load_2d(sm + i * A_BYTES, &maps.w, &full[i], (kb0 + i) * f4::KSB, n0);
+                tma_load_2d(sm_s + i * SF, &maps.ws, &full[i], (kb0 + i) * (SF / 8), blockIdx.x);
+            }
+            tma_prefetch_desc(&maps.x), tma_prefetch_desc(&maps.xs);
         }
-        tma_prefetch_desc(&maps.x), tma_prefetch_desc(&maps.xs);
     }
     if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
     tc_fence_before();
@@ -193,42 +260,52 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
             grid_launch_dependents();
             for (int i = 0; i < nk; ++i) {
                 const int s = i % STAGES, kb = kb0 + i;
-                if (i >= STAGES) {
-                    if (!mbar_wait(&empty[s], ((i / STAGES) - 1) & 1, actx, kErrWaitEmpty)) break;
+                if (i >= STAGES && !mbar_wait(&empty[s], ((i / STAGES) - 1) & 1, actx, kErrWaitEmpty)) break;
+                if (FUSED || i >= STAGES) {
                     mbar_expect_tx(&full[s], STAGE_BYTES);
                     tma_load_2d(sm + s * A_BYTES, &maps.w, &full[s], kb * f4::KSB, n0);
-                    tma_load_2d(sm_s + s * 2 * SF, &maps.ws, &full[s], kb * (SF / 8), blockIdx.x);
+                    tma_load_2d(sm_s + s * SF, &maps.ws, &full[s], kb * (SF / 8), blockIdx.x);
                 }
-                tma_load_2d(sm_b + s * BN * f4::KSB, &maps.x, &full[s], kb * f4::KSB, m0);
-                tma_load_2d(sm_s + s * 2 * SF + SF, &maps.xs, &full[s], kb * (SF / 8), m0 / 128);
+                if constexpr (!FUSED) {
+                    tma_load_2d(sm_b + s * BN * f4::KSB, &maps.x, &full[s], kb * f4::KSB, m0);
+                    tma_load_2d(sm_t + s * SF, &maps.xs, &full[s], kb * (SF / 8), m0 / 128);
+                }
             }
         }
     } else if (warp == 1) {
         if (elect_lane()) {
-            bool ok = true;
-            for (int i = 0; i < nk; ++i) {
-                const int s = i % STAGES;
+            bool ok = !FUSED || mbar_wait_hot(tokens_full, 0, actx, kErrWaitFull);
+            for (int i = 0; ok && i < nk; ++i) {
+                const int s = i % STAGES, t = FUSED ? i : s;
                 if (!mbar_wait_hot(&full[s], (i / STAGES) & 1, actx, kErrWaitFull)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint64_t sf = scale_desc(smem_u32(sm_s + s * 2 * SF));
                 issue_stage<FORMAT, 1, BM, BN, 1>(tmem, make_sw128_kmajor_desc(smem_u32(sm + s * A_BYTES)),
-                                                  make_sw128_kmajor_desc(smem_u32(sm_b + s * BN * f4::KSB)), tmem + BN + s * sf_cols(FORMAT), sf,
-                                                  sf + (uint64_t)(SF >> 4), (p.K - (kb0 + i) * f4::KS + 63) / 64, i == 0);
+                                                  make_sw128_kmajor_desc(smem_u32(sm_b + t * BN * f4::KSB)), tmem + BN + s * sf_cols(FORMAT),
+                                                  scale_desc(smem_u32(sm_s + s * SF)), scale_desc(smem_u32(sm_t + t * SF)),
+                                                  (p.K - (kb0 + i) * f4::KS + 63) / 64, i == 0);
                 tc_commit(&empty[s]);
             }
             if (ok) tc_commit(acc_full);
         }
     } else {
+        if constexpr (FUSED) {
+            grid_dependency_wait();
+            quantise_tokens<FORMAT, T>(static_cast<const T*>(p.x), p.ldx, rows, p.K, kb0, nk, sm_b, sm_t, s_xg,
+                                       reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(full) + f4::BAR_BYTES / 2));
+        }
         if (n < p.N) {
             if (p.wg) gw = p.wg[n];
             if (p.bias) bias = to_f<T>(static_cast<const T*>(p.bias)[n]);
         }
-        grid_dependency_wait();
-        for (int t = tid - 64; t < rows; t += 32 * EW) s_xg[t] = p.xg ? p.xg[m0 + t] : 1.0f;
+        if constexpr (!FUSED) {
+            grid_dependency_wait();
+            for (int t = tid - 64; t < rows; t += 32 * EW) s_xg[t] = p.xg ? p.xg[m0 + t] : 1.0f;
+        }
         asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (FUSED && tid == 64) mbar_arrive(tokens_full);
         bool ok = true;
         if (lane == 0) ok = mbar_wait(acc_full, 0, actx, kErrWaitDFull);
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -600,15 +677,17 @@ static int stream_splits(int64_t tiles, int stages) {
     return splits;
 }
 
-template <int FORMAT, typename T, int BN, bool DEEP>
+template <int FORMAT, typename T, int BN, bool DEEP, bool FUSED = false>
 static int launch_stream(const void* w, const void* ws, const void* xq, const void* xs, Fp4Args a, cudaStream_t st) {
     Fp4Maps m{};
     if (int e = make_tmap_2d(&m.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.N, a.K / 2, fs::BM, f4::KSB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
-    if (int e = make_tmap_2d(&m.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, a.M, a.K / 2, BN, f4::KSB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
     if (int e = make_tmap_scales(&m.ws, ws, a.N, a.K, FORMAT, 1)) return e;
-    if (int e = make_tmap_scales(&m.xs, xs, a.M, a.K, FORMAT, 1)) return e;
-    auto kernel = fp4_stream_kernel<FORMAT, T, BN, DEEP>;
-    constexpr int smem = fs::smem_bytes(FORMAT, BN, DEEP);
+    if constexpr (!FUSED) {
+        if (int e = make_tmap_2d(&m.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, xq, a.M, a.K / 2, BN, f4::KSB, CU_TENSOR_MAP_SWIZZLE_128B)) return e;
+        if (int e = make_tmap_scales(&m.xs, xs, a.M, a.K, FORMAT, 1)) return e;
+    }
+    auto kernel = fp4_stream_kernel<FORMAT, T, BN, DEEP, FUSED>;
+    constexpr int smem = fs::smem_bytes(FORMAT, BN, DEEP, FUSED);
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     RWKV7_REQUIRE(e == cudaSuccess, RWKV7_ERR_CUDA, "fp4_linear: %s", cudaGetErrorString(e));
     const int tn = (a.N + fs::BM - 1) / fs::BM, tm = (a.M + BN - 1) / BN;
@@ -650,6 +729,17 @@ static int launch_pair(const void* w, const void* ws, const void* xq, const void
     const cudaError_t l = launch_programmatic(kernel, dim3(2 * pairs), dim3(fp::THREADS), smem, st, m, a);
     RWKV7_REQUIRE(l == cudaSuccess, RWKV7_ERR_CUDA, "fp4_linear: %s", cudaGetErrorString(l));
     return check_launch("fp4_pair_kernel");
+}
+
+// Whether the product quantises its tokens itself, one launch less: few of them, a grid of one CTA an SM, a K range a CTA that fits.  Every CTA
+// then quantises its range of K again, which is worth it while there is little of it: by tokens x stages.  us with the quantiser / without, weights out
+// of memory, nvfp4: 1 x 4096 -> 16384 (16) 11.0 / 9.6, 1 x 10240 -> 2560 (10) 9.1 / 8.3, 4 x 4096 -> 4096 (16) 7.0 / 7.0, 4 x 768 -> 768 (12) 4.5 / 4.1, 8 x 768 -> 768 (24)
+// 4.5 / 4.8, 2 x 4096 -> 16384 (32) 11.2 / 11.5; mxfp4, which needs no largest magnitude of the row: 1 x 4096 -> 16384 10.8 / 8.6, 4 x 16384 -> 4096 (64)
+// 12.8 / 11.8, 4 x 4096 -> 16384 (64) 10.9 / 10.9, 8 x 2560 -> 10240 (80) 7.3 / 7.9.  A call costs the host 13.1 us instead of 15.7.
+static bool quantises_itself(int M, int K, int N, int format) {
+    const int tiles = (N + fs::BM - 1) / fs::BM, stages = (K + f4::KS - 1) / f4::KS, splits = stream_splits(tiles, stages);
+    const int range = (stages + splits - 1) / splits;
+    return M <= 16 && tiles <= kSMs && range <= fs::FUSED_STAGES && M * range <= (format == fp4::MX ? 64 : 16);
 }
 
 template <int FORMAT, typename T>
@@ -715,8 +805,11 @@ extern "C" int rwkv7_fp4_linear(const void* x, int64_t ldx, const void* w_packed
     uint8_t* base = static_cast<uint8_t*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     float* xg = reinterpret_cast<float*>(base + ws.row_scale);
-    if (int e = launch_fp4_quant(x, ldx, base, base + ws.scales, xg, M, K, format, dtype, st)) return e;
+    const bool fused = quantises_itself(M, K, N, format);
+    if (!fused)
+        if (int e = launch_fp4_quant(x, ldx, base, base + ws.scales, xg, M, K, format, dtype, st)) return e;
     Fp4Args a{};
+    a.x = x, a.ldx = ldx;
     a.wg = w_row_scale, a.xg = format == fp4::NV ? xg : nullptr;
     a.bias = bias, a.residual = residual, a.y = y;
     a.M = M, a.N = N, a.K = K, a.relu2 = epilogue == RWKV7_EPI_RELU2;
@@ -724,6 +817,9 @@ extern "C" int rwkv7_fp4_linear(const void* x, int64_t ldx, const void* w_packed
     a.error = kernel_error_word();
     RWKV7_REQUIRE(a.error != nullptr, RWKV7_ERR_CUDA, "fp4_linear: cannot resolve the device error word");
     RWKV7_DISPATCH_DTYPE(dtype, T, {
+        if (fused)
+            return format == fp4::MX ? launch_stream<fp4::MX, T, 16, true, true>(w_packed, w_scales, nullptr, nullptr, a, st)
+                                     : launch_stream<fp4::NV, T, 16, true, true>(w_packed, w_scales, nullptr, nullptr, a, st);
         return format == fp4::MX ? dispatch_fp4<fp4::MX, T>(w_packed, w_scales, base, base + ws.scales, a, st)
                                  : dispatch_fp4<fp4::NV, T>(w_packed, w_scales, base, base + ws.scales, a, st);
     });

@@ -171,7 +171,7 @@ def fp4_linear(x, packed, scales, row_scale=None, bias=None, *, format: str = "n
         ws = packed.new_empty(nbytes)
         epi = _lib.EPI_RELU2 if relu2 else _lib.EPI_NONE if residual is None else _lib.EPI_ADD
         _lib.check(_lib.lib.rwkv7_fp4_linear(x2.data_ptr(), ld, packed.data_ptr(), scales.data_ptr(), ptr(row_scale), ptr(bias), ptr(residual),
-                                             out.data_ptr(), ws.data_ptr(), nbytes, M, K, N, epi, f, dt, stream_ptr(x2)), "fp4_linear", 2)
+                                             out.data_ptr(), ws.data_ptr(), nbytes, M, K, N, epi, f, dt, stream_ptr(x2)), "fp4_linear")
     return out
 
 

@@ -480,8 +480,9 @@ int rwkv7_fp4_quant(const void* x, int64_t ldx, void* packed, void* scales, floa
                     void* stream);
 int rwkv7_fp4_dequant(const void* packed, const void* scales, const float* row_scale, void* out, int rows, int K, int format, int dtype,
                       void* stream);
-/* y [M,N] = epilogue(x_q [M,K] . w_q [N,K]^T (+ bias)): x is quantised on the way (rwkv7_fp4_quant into the workspace), both
- * operands stay in 4 bits on the tensor cores, sums are fp32 and rounded once after the epilogue (relu(.)^2, or + residual).
+/* y [M,N] = epilogue(x_q [M,K] . w_q [N,K]^T (+ bias)): x is quantised on the way (rwkv7_fp4_quant into the workspace, or
+ * the product itself where tokens are few), both operands stay in 4 bits on the tensor cores, sums are fp32 and rounded once after the
+ * epilogue (relu(.)^2, or + residual).
  * w_row_scale NULL = 1. */
 int64_t rwkv7_fp4_linear_workspace_bytes(int M, int K, int format);
 int rwkv7_fp4_linear(const void* x, int64_t ldx, const void* w_packed, const void* w_scales, const float* w_row_scale,

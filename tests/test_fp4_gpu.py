@@ -105,6 +105,28 @@ def test_linear_against_64_bits(fmt, dtype, m, k, n):
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("m,k,n", [(1, 96, 130), (1, 4128, 1000), (2, 2560, 257), (3, 32, 5), (4, 800, 300), (5, 768, 768), (7, 544, 128),
+                                   (9, 288, 65), (16, 96, 200), (16, 1056, 384), (4, 16384, 2048)])
+def test_few_tokens_of_different_sizes(fmt, dtype, m, k, n):
+    """Rows apart by orders of magnitude, one of zeros, one with a single large element at its end, a row stride that is not K; the
+    weight is made right before the product that reads it."""
+    x = rnd(m, k + 64, seed=m + k) * torch.exp2(torch.arange(m, device="cuda") % 5 * 2.0 - 4)[:, None]
+    x[m // 2, k - 1] = 300
+    if m > 2:
+        x[1] = 0
+    x = x.to(DT[dtype])[:, :k]
+    w = rnd(n, k, seed=n, scale=k ** -0.5)
+    xv, wv = values64(x.contiguous(), fmt), values64(w, fmt)
+    want = xv @ wv.t()
+    err, rel, tiny = bound(xv, wv, want, dtype)
+    for _ in range(3):
+        y = hb.fp4_linear(x, *hb.quantize_fp4(w, fmt), format=fmt)
+        assert float(((y.double() - want).abs() - (err + rel * want.abs() + tiny)).max()) <= 0
+    assert _lib.kernel_status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 @pytest.mark.parametrize("m", [3, 70, 600])
 def test_a_bad_element_stays_in_its_row(fmt, m):
     """A row with a NaN or an infinity gives a row of NaN; a weight's gives a column; everything else keeps its bits."""
