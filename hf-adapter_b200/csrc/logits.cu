@@ -521,40 +521,42 @@ __device__ __noinline__ lg::Cut descend(const float* zs, int slice, int first, f
 }
 
 // ------------------------------ a window of bins around the cut, sorted
-// Which bins go on the list of the first CTA, in s.window_first, s.window_last (first > last: not even the cut's bin fits).
-// `exact`: the cut is in this bin, else it may be in the two on either side.  From the first bin if no more than `room` tokens may be
-// kept (and, as sorting so few costs the same, as many bins as hold FEW where the cut is not exact: where tokens are few they are heavy,
-// and a cut that is missed by one may be many bins away), else around the cut alone: what lies above is then weighed and raced in passing, not sorted.
-__device__ __forceinline__ void place_window(lg::Shared& s, int bin, bool exact, unsigned int room) {
+// Where a cut lies: its bin is known (by count), or the estimate is in the middle of it, towards its first or its last token, or
+// the bin holds too few tokens to tell.
+enum Where { kAround = 0, kHere = 1, kBefore = 2, kAfter = 3 };
+// Which bins go on the list of the first CTA, in s.window_first, s.window_last (first > last: not even the cut's bin fits).  From the
+// first bin if no more than `room` tokens may be kept, and then two bins more where the cut is estimated, and (as sorting so few costs the same) as many as
+// hold FEW: where tokens are few they are heavy, and a cut that is missed by one may be many bins away.  Else the cut's bin, with its neighbours where it may
+// lie there: what lies above is weighed and raced in passing, not sorted.
+__device__ __forceinline__ void place_window(lg::Shared& s, int bin, int where, bool exact, unsigned int room) {
     if (threadIdx.x == 0) {
         const int wide = exact ? bin : min(bin + 2, lg::BINS - 1);
-        int first = 0, last = wide;
+        int first = 0, last = max(wide, exact ? 0 : s.reach);
         if (s.upto[wide] > room) {
-            first = exact ? bin : max(bin - 2, 0);
+            first = where == kAround ? max(bin - 2, 0) : where == kBefore ? max(bin - 1, 0) : bin;
+            last = where == kAround ? wide : where == kAfter ? min(bin + 1, lg::BINS - 1) : bin;
             auto tokens = [&] { return s.upto[last] - (first ? s.upto[first - 1] : 0); };
             while (first <= last && tokens() > lg::LIST) {
                 if (last > bin) --last;
                 else ++first;
             }
-        } else if (!exact) {
-            last = max(wide, s.reach);
         }
         s.window_first = first, s.window_last = last;
     }
     __syncthreads();
 }
-// The cut's bin (s.bin) and the window.  The bin is known by count (k > 0), or
+// The cut's bin (s.bin: 4 * bin + where) and the window.  The bin is known by count (k > 0), or
 // estimated: a bin's mass is taken as its count times e of its middle (1.6 % off at most).  Few heavy tokens make most of that
 // error, above the cut, so what the estimate of the whole row is off by (`all`: the row's mass) is taken as the error at the cut too (of 64 rows of
-// normal logits 4 missed the window without this); two bins on either side allow for the rest.  The exact masses decide later.
+// normal logits 4 missed a window of five bins without this); `where` says which neighbours the rest may reach.  The exact masses decide later.
 __device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, float want, float all, unsigned int room) {
     static_assert(lg::BINS == 2 * lg::THREADS, "two bins a thread");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = 2 * threadIdx.x;
-    if (threadIdx.x == 0) s.bin = lg::BINS - 1;
+    if (threadIdx.x == 0) s.bin = 4 * (lg::BINS - 1) + kAround;
     __syncthreads();
     if (k) {
         const unsigned int before = b ? s.upto[b - 1] : 0;
-        if (before < k && s.upto[b + 1] >= k) s.bin = s.upto[b] >= k ? b : b + 1;
+        if (before < k && s.upto[b + 1] >= k) s.bin = 4 * (s.upto[b] >= k ? b : b + 1) + kHere;
     } else {
         const unsigned int n0 = s.upto[b] - (b ? s.upto[b - 1] : 0), n1 = s.upto[b + 1] - s.upto[b];
         const float middle = expf(-((float)b + 0.5f) / lg::BIN_SCALE), q0 = (float)n0 * middle;
@@ -577,10 +579,16 @@ __device__ __forceinline__ void choose_window(lg::Shared& s, unsigned int k, flo
         // rounding makes it two, the first, in every CTA)
         q += upto;
         const float left = __shfl_up_sync(0xffffffffu, q, 1), before = lane ? left : upto;
-        if (before < want && q >= want) atomicMin(&s.bin, before + q0 >= want ? b : b + 1);
+        if (before < want && q >= want) {
+            // what is left of the estimate's error is some hundredths of a bin that holds tokens enough
+            const bool one = before + q0 >= want;
+            const float part = one ? (want - before) / q0 : (want - before - q0) / q1;
+            const int where = (one ? n0 : n1) < 16 ? kAround : part < 0.2f ? kBefore : part > 0.8f ? kAfter : kHere;
+            atomicMin(&s.bin, 4 * (one ? b : b + 1) + where);
+        }
     }
     __syncthreads();
-    place_window(s, s.bin, k != 0, room);
+    place_window(s, s.bin >> 2, s.bin & 3, k != 0, room);
 }
 
 // list[0, n) ascending, n at most LIST; what pads it to a power of two is the largest key
@@ -589,29 +597,20 @@ __device__ __forceinline__ void sort_list(lg::u64* list, int n) {
     while (size < n) size *= 2;
     for (int i = n + threadIdx.x; i < size; i += lg::THREADS) list[i] = ~0ull;
     __syncthreads();
-    if (size <= 64) {  // one warp, a pair a lane: no barrier between the steps (50 tokens: 4600 -> 1300 cycles)
-        if (threadIdx.x < 32)
-            for (int span = 2; span <= size; span *= 2)
-                for (int d = span / 2; d > 0; d /= 2) {
-                    const int t = threadIdx.x, i = 2 * t - (t & (d - 1));
-                    if (t < size / 2) {
-                        const lg::u64 a = list[i], b = list[i + d];
-                        if ((a > b) == ((i & span) == 0)) list[i] = b, list[i + d] = a;
-                    }
-                    __syncwarp();
-                }
-        __syncthreads();
-        return;
-    }
-    for (int span = 2; span <= size; span *= 2)
-        for (int d = span / 2; d > 0; d /= 2) {
-            for (int t = threadIdx.x; t < size / 2; t += lg::THREADS) {
+    // a pair a thread, who meet without the others: one warp up to 64 tokens (50: 4600 -> 1300 cycles), a barrier of their own above
+    const int t = threadIdx.x, threads = size / 2 < 32 ? 32 : size / 2;
+    if (t < threads)
+        for (int span = 2; span <= size; span *= 2)
+            for (int d = span / 2; d > 0; d /= 2) {
                 const int i = 2 * t - (t & (d - 1));
-                const lg::u64 a = list[i], b = list[i + d];
-                if ((a > b) == ((i & span) == 0)) list[i] = b, list[i + d] = a;
+                if (t < size / 2) {
+                    const lg::u64 a = list[i], b = list[i + d];
+                    if ((a > b) == ((i & span) == 0)) list[i] = b, list[i + d] = a;
+                }
+                if (threads == 32) __syncwarp();
+                else asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
             }
-            __syncthreads();
-        }
+    __syncthreads();
 }
 
 // what the two places of this thread on the sorted list hold, and the mass before them
@@ -1006,8 +1005,8 @@ __global__ void __launch_bounds__(lg::THREADS, 2) pick_kernel(const T* __restric
 // Rows with filters.  The cuts are found by counts in 1024 bins of m - z (and by what the bins weigh, estimated), which single out a
 // window of some hundred tokens; those alone are sorted, by the first CTA, with exact masses.  A row is in shared memory from the first pass
 // on.  Some 20 steps that wait for one another (barriers of CTA and cluster, a sort) bound it, for many rows the same with two CTAs an SM.  Device us, 65536
-// tokens fp16 with log-probability, one row / 64 / 256 rows: top-k 50 15.5 / 23.3 / 80, and with top-p the same; top-p 0.9 where 24 tokens are
-// likely 15.7 / 23.5 / 82; top-p 0.9 of normal logits (2400 tokens kept) 25 / 38 / 135; min-p 8.7 / 15 / 54; a flat row, which no
+// tokens fp16 with log-probability, one row / 64 / 256 rows: top-k 50 15.6 / 23.5 / 80, and with top-p the same; top-p 0.9 where 24 tokens are
+// likely 16 / 24 / 83; top-p 0.9 of normal logits (2400 tokens kept) 21 / 34 / 124; min-p 8.7 / 15 / 54; a flat row, which no
 // window holds, 47 / 94 / 350.
 template <typename T, bool RULES>
 __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restrict__ logits, int64_t ld, const rwkv7_logit_rules rules,
@@ -1091,13 +1090,14 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
         for (int stage = by_k && (unsigned int)k < s.upto[BINS - 1] ? 0 : 1; stage < (by_p ? 2 : 1); ++stage) {
             if (stage == 1 && cut_k.found) target_p = share_of(share, (double)cut_k.mass);
             // The last cut's list is short rather than whole: us of one row, top-k 500 / 900 with the whole list 20.2 / 23.4, around the cut 17.7 /
-            // 18.1 (64 rows 33.8 / 37.0, 28.4 / 29.9), equal up to 128 tokens.  For top-k before top-p it is whole where that is possible, which
-            // saves the second list: top-k 500 then top-p one row 19.8, two lists 26.7.
+            // 18.0 (64 rows 33.8 / 37.0, 28.6 / 29.2), equal up to 128 tokens.  For top-k before top-p it is whole where that is possible, which
+            // saves the second list: top-k 500 then top-p one row 20.2, two lists 26.7.
             const bool last = stage == 1 || !by_p;
             const unsigned int room = last ? 128 : LIST;
             choose_window(s, stage == 0 ? (unsigned int)k : 0u, (float)((double)target_p / MASS_UNIT), (float)all, room);
             // where the descent looks first if there is no list
-            int r0 = stage == 0 ? s.bin : max(s.bin - 2, 0), r1 = stage == 0 ? s.bin : min(s.bin + 2, BINS - 1);
+            const int cut_bin = s.bin >> 2;
+            int r0 = stage == 0 ? cut_bin : max(cut_bin - 2, 0), r1 = stage == 0 ? cut_bin : min(cut_bin + 2, BINS - 1);
             bool done = false;
 #pragma unroll 1
             for (int turn = 2 * stage; turn < 2 * stage + 2 && !done; ++turn) {
@@ -1161,7 +1161,7 @@ __global__ void __launch_bounds__(lg::THREADS, 2) filter_kernel(const T* __restr
                     const int bin = before ? w0 - 1 : min(w1 + 1, BINS - 1);
                     r0 = before ? max(bin - 3, 0) : bin, r1 = before ? bin : min(bin + 3, BINS - 1);
                     __syncthreads();
-                    place_window(s, bin, false, room);
+                    place_window(s, bin, kAround, false, room);
                 }
             }
             if (!done) {

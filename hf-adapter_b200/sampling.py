@@ -124,7 +124,7 @@ def process_logits(logits, *, tokens=None, lengths=None, prompt_lengths=None, re
                allowed)
     out_ld = V
     if out is None:
-        out = logits.new_empty((B, V))
+        out = torch.empty_like(logits)
     else:
         out_ld = out.stride(0) if B > 1 and out.dim() == 2 else V
         if (out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != dev or (V > 1 and out.stride(1) != 1)
