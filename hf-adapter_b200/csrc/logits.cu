@@ -9,7 +9,8 @@
 //   min-p  keeps e >= min_p;
 //   token  = argmax of e / noise over what is kept (noise: independent Exp(1) variates, which makes it a draw from the
 //            renormalised distribution); temperature <= 0: argmax of z.  The lowest index wins a tie.
-// A NaN is never drawn, +inf counts as the largest finite number; a row without any token gives -1.
+// A NaN is never drawn, +inf counts as the largest finite number, and a quotient beyond it as the finite number at that end (a row
+// of the type's lowest value is a row of equal tokens, not an empty one); a row without any token gives -1.
 //
 // A history is counted in shared memory, a word a token of the slice that a CTA holds (bit 31: in the prompt; below: times
 // generated): integer atomics, so the order does not matter.  Every sum that is not of integers runs in a fixed order, and
@@ -766,7 +767,7 @@ __device__ __forceinline__ Draw row_draw(const rwkv7_draw_params& d, bool noise,
 __device__ __forceinline__ float over_temperature(float x, float t, float inv) {
     const float q = x * inv;
     float z = fmaf(fmaf(-q, t, x), inv, q) + 0.0f;  // (-0 becomes 0)
-    if (!(fabsf(q) < 1e37f)) z = x > -INFINITY ? fminf(x / t, lg::FLOAT_MAX) : -INFINITY;  // (NaN compares false)
+    if (!(fabsf(q) < 1e37f)) z = x > -INFINITY ? fmaxf(fminf(x / t, lg::FLOAT_MAX), -lg::FLOAT_MAX) : -INFINITY;  // (NaN compares false)
     return z;
 }
 

@@ -251,6 +251,24 @@ def test_values_that_are_not_finite_and_empty_rows():
     assert int(hb.sample_tokens(torch.zeros(1, 4, device="cuda"), odd * nan)) == 0
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_rows_of_the_lowest_value(dtype):
+    """A mask of the type's lowest number instead of -inf: beside other values it takes all probability away, alone it is a row of
+    equal tokens, at every temperature."""
+    V, low = 5000, torch.finfo(DT[dtype]).min
+    z = torch.full((3, V), low, device="cuda", dtype=DT[dtype])
+    z[1, 4000:4003] = 1
+    z[2, ::2] = -float("inf")
+    noise = noise_for(3, V, seed=3)
+    want = [int(noise[0].argmin()), 4000 + int(noise[1, 4000:4003].argmin()), 1 + 2 * int(noise[2, 1::2].argmin())]
+    for T in (0.25, 1.0, 4.0):
+        for kw in (dict(), dict(top_k=V - 1), dict(min_p=0.5), dict(top_p=0.9999999, min_p=0.1)):
+            tok, lp = hb.sample_tokens(z, noise, temperature=T, return_logprobs=True, **kw)
+            assert tok.tolist() == want, (T, kw)
+            assert torch.allclose(lp.cpu(), -torch.log(torch.tensor([5000.0, 3.0, 2500.0])), atol=1e-5)
+    assert hb.sample_tokens(z).tolist() == [0, 4000, 1]
+
+
 def test_close_values_in_one_bin():
     """Thousands of neighbouring floats between the cuts: the search has to go down to single keys."""
     V = 30000
