@@ -5,10 +5,11 @@
 //   nvfp4: g = 2^(floor(log2 amax of the row) - 10) (1 for a row of zeros), s = e4m3(amax of the block / g / 6),
 //          code = e2m1(x / g / s), 0 where s is 0.  amax / g / 6 stays below 342, inside E4M3's 448.
 //
-// Every rounding is to nearest, ties to even: powers of two divide exactly; x / s is formed as a product with 1 / s and one
-// correction step, which is the correctly rounded quotient; a sixth is taken as the product with the fp32 nearest to 1 / 6,
-// 2^-25 off, so six times a number of few bits gives that number.  For fp16 / bf16 input a tie is therefore met exactly or missed
-// by 2^-12 at least; fp32 input can round the other way where the quotient is within 2^-23 of one.
+// Every rounding is to nearest, ties to even: powers of two divide exactly; x / s is formed as a product with 1 / s and, for fp32,
+// one correction step, which makes it the correctly rounded quotient, for 16 bits rounded to steps of 2^-17 instead; a sixth is
+// taken as the product with the fp32 nearest to 1 / 6, 2^-25 off, so six times a number of few bits gives that number.  For
+// fp16 / bf16 input a tie is therefore met exactly or missed by 2^-12 at least; fp32 input can round the other way where the
+// quotient is within 2^-23 of one.
 // A block with an element that is not finite gets a NaN scale; the row's largest magnitude is taken over the finite
 // ones.
 #include "fp4_encode.cuh"
@@ -29,7 +30,7 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
 
 // `team` threads a row, P pieces of 16 elements a thread, read once and kept (P = 0: read again for the codes).  Rows beyond R
 // pad the last scale tile with zeros.  Bound by the memory for many rows, where nvfp4 also waits for the row's maximum before its first code: 8192 x 4096
-// bf16 (67 MB in, 18 to 19 out) mxfp4 14.8 us = 5.7 TB/s, nvfp4 20.9 us = 4.1 TB/s; by the launch for few: 1 x 768 1.3 and 1.8 us, 64 x 4096 1.7 and 2.1.
+// bf16 (67 MB in, 18 to 19 out) mxfp4 14.8 us = 5.7 TB/s, nvfp4 18.8 us = 4.6 TB/s; by the launch for few: 1 x 768 1.3 and 1.8 us, 64 x 4096 1.7 and 2.1.
 template <typename T, int FORMAT, int P>
 __global__ void __launch_bounds__(256) fp4_quant_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ packed,
                                                         uint8_t* __restrict__ scales, float* __restrict__ row_scale, int R, int K, int team) {
@@ -42,6 +43,7 @@ __global__ void __launch_bounds__(256) fp4_quant_kernel(const T* __restrict__ x,
     grid_launch_dependents();
     const T* xr = x + row * ldx;
     Piece<T> kept[P ? P : 1];
+    float most[P ? P : 1];
     if constexpr (P > 0) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
@@ -55,9 +57,12 @@ __global__ void __launch_bounds__(256) fp4_quant_kernel(const T* __restrict__ x,
         float m = 0.0f;
         if constexpr (P > 0) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) m = fmaxf(m, finite_amax(kept[i]));
+            for (int i = 0; i < P; ++i) most[i] = piece_amax(kept[i]), m = fmaxf(m, finite_amax(kept[i], most[i]));
         } else {
-            for (int p = at; p < pieces; p += team) m = fmaxf(m, finite_amax(load_piece<T>(xr + 16 * p)));
+            for (int p = at; p < pieces; p += team) {
+                const Piece<T> one = load_piece<T>(xr + 16 * p);
+                m = fmaxf(m, finite_amax(one, piece_amax(one)));
+            }
         }
         m = group_max<32>(m);
         if (team > 32) {
@@ -69,9 +74,9 @@ __global__ void __launch_bounds__(256) fp4_quant_kernel(const T* __restrict__ x,
         ge = m > 0.0f ? max(e - 10, 1) : 127;
         if (at == 0 && row < R) row_scale[row] = __int_as_float(ge << 23);
     }
-    const auto put = [&](const Piece<T>& piece, int p) {
+    const auto put = [&](const Piece<T>& piece, float m, int p) {
         uint2 codes;
-        uint32_t byte = encode_piece<T, FORMAT>(piece, ge, codes);
+        uint32_t byte = encode_piece<T, FORMAT>(piece, m, ge, codes);
         if (p < pieces) *reinterpret_cast<uint2*>(packed + row * (K / 2) + 8 * p) = codes;
         else byte = 0;
         // four scales to one word: blocks lie one (nvfp4) or two (mxfp4) lanes apart
@@ -83,13 +88,13 @@ __global__ void __launch_bounds__(256) fp4_quant_kernel(const T* __restrict__ x,
     if constexpr (P > 0) {
 #pragma unroll
         for (int i = 0; i < P; ++i)
-            if (at - lane + i * team < padded) put(kept[i], at + i * team);  // (whole warps, for the shuffles)
+            if (at - lane + i * team < padded) put(kept[i], FORMAT == NV ? most[i] : piece_amax(kept[i]), at + i * team);  // (whole warps, for the shuffles)
     } else {
         for (int p0 = at - lane; p0 < padded; p0 += team) {
             const int p = p0 + lane;
             Piece<T> one{};
             if (p < pieces) one = load_piece<T>(xr + 16 * p);
-            put(one, p);
+            put(one, piece_amax(one), p);
         }
     }
 }

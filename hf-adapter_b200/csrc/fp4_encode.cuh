@@ -64,9 +64,8 @@ template <typename T> __device__ __forceinline__ float piece_amax(const Piece<T>
         return max_nan(to_f<T>(m.x), to_f<T>(m.y));
     }
 }
-// the same over the finite elements alone
-template <typename T> __device__ __forceinline__ float finite_amax(const Piece<T>& p) {
-    float m = piece_amax(p);
+// the same over the finite elements alone; m: piece_amax(p)
+template <typename T> __device__ __forceinline__ float finite_amax(const Piece<T>& p, float m) {
     if (!(m < INFINITY)) {
         float v[16];
         widen(p, v);
@@ -78,12 +77,11 @@ template <typename T> __device__ __forceinline__ float finite_amax(const Piece<T
     return m;
 }
 
-// Codes and the block's scale byte of one piece; g's exponent byte, inv_g = 1 / g (nvfp4).  Whole warps.
+// Codes and the block's scale byte of one piece; m: piece_amax(piece), ge: g's exponent byte (nvfp4).  Whole warps.
 template <typename T, int FORMAT>
-__device__ __forceinline__ uint32_t encode_piece(const Piece<T>& piece, int ge, uint2& codes) {
+__device__ __forceinline__ uint32_t encode_piece(const Piece<T>& piece, float m, int ge, uint2& codes) {
     float v[16];
     widen(piece, v);
-    float m = piece_amax(piece);
     uint32_t byte;
     if constexpr (FORMAT == MX) {
         m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
@@ -103,10 +101,17 @@ __device__ __forceinline__ uint32_t encode_piece(const Piece<T>& piece, int ge, 
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i] *= inv_g;
         }
+        if constexpr (sizeof(T) == 2) {
+            // x / s misses a tie by 2^-12 of it at least, or is one, and is at most 9: rounded to steps of 2^-17 it is on the same side, or on it
+            // (8192 x 4096 18.8 us with this and one amax a piece, 20.9 with the quotient's correction step and two)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float q = v[i] * inv;
-            v[i] = fmaf(fmaf(-q, s, v[i]), inv, q);
+            for (int i = 0; i < 16; ++i) v[i] = fmaf(v[i], inv, 96.0f) - 96.0f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float q = v[i] * inv;
+                v[i] = fmaf(fmaf(-q, s, v[i]), inv, q);
+            }
         }
     }
     float lo[8], hi[8];

@@ -142,7 +142,10 @@ __device__ __forceinline__ void quantise_tokens(const T* x, int64_t ldx, int M, 
         if constexpr (FORMAT == fp4::NV) {
             float m = 0.0f;
 #pragma unroll 4
-            for (int p = at; p < pieces; p += team) m = fmaxf(m, finite_amax(load_piece<T>(xr + 16 * p)));
+            for (int p = at; p < pieces; p += team) {
+                const Piece<T> one = load_piece<T>(xr + 16 * p);
+                m = fmaxf(m, finite_amax(one, piece_amax(one)));
+            }
             m = group_max<32>(m);
             if (team > 32) {
                 asm volatile("bar.sync 1, 256;" ::: "memory");  // (the last rows' maxima have been read)
@@ -162,7 +165,7 @@ __device__ __forceinline__ void quantise_tokens(const T* x, int64_t ldx, int M, 
             Piece<T> piece{};
             if (p < pieces) piece = load_piece<T>(xr + 16 * p);
             uint2 c;
-            const uint32_t byte = encode_piece<T, FORMAT>(piece, ge, c);
+            const uint32_t byte = encode_piece<T, FORMAT>(piece, piece_amax(piece), ge, c);
             if (live && i < 16 * nk) {
                 const int stage = i >> 4, j = i & 15;  // a piece: 8 bytes of the row's 128
                 *reinterpret_cast<uint2*>(codes + stage * (BN * f4::KSB) + row * f4::KSB + (((j >> 1) ^ (row & 7)) << 4) + (j & 1) * 8) = c;

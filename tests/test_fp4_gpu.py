@@ -47,6 +47,32 @@ def test_quantiser_bits(fmt, dtype, rows, k):
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_ties_and_their_neighbours(fmt, dtype):
+    """Every half-way point between two codes, and the numbers of the type on both sides of it, under every mantissa of a scale."""
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64)
+    rows = []
+    for e in range(-5, 6):
+        for mantissa in range(8, 16):
+            s = mantissa / 8 * 2.0 ** e
+            exact = (ties * s).to(DT[dtype])  # (3 + 4 bits: exact)
+            assert torch.equal(exact.double(), ties * s)
+            up, down = torch.nextafter(exact, exact + 1000), torch.nextafter(exact, exact - 1000)
+            top = torch.tensor([6 * s], dtype=DT[dtype])
+            rows.append(torch.cat([torch.cat((top, v, -v, top)) for v in (exact, up, down, exact)]))
+    x = torch.stack(rows).cuda()
+    got, want = hb.quantize_fp4(x, fmt), hb.quantize_fp4_weight(x, fmt)
+    drop = lambda p: torch.stack([torch.where(n & 7 == 0, 0, n) for n in (p & 15, p >> 4)])
+    assert torch.equal(got[1], want[1]) and torch.equal(drop(got[0]), drop(want[0]))
+    # and the product of few tokens, which quantises them itself: one channel a code position picks the values out
+    if x.shape[1] == 64:
+        w = hb.quantize_fp4(torch.eye(64, device="cuda"), fmt)
+        for r in range(0, x.shape[0], 16):
+            few, many = hb.fp4_linear(x[r:r + 4], *w, format=fmt), hb.fp4_linear(x, *w, format=fmt)[r:r + 4]
+            assert torch.equal(few, many)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 def test_quantiser_extremes(fmt):
     """Zeros, subnormals, the largest numbers, values that are not finite; strided and unaligned rows."""
     x = torch.zeros(8, 64, device="cuda")
