@@ -107,14 +107,14 @@ __device__ __forceinline__ void issue_stage(uint32_t d, uint64_t da, uint64_t db
 
 // ---------------------------------------------------------------- few tokens
 namespace fs {
-constexpr int BM = 128, EW = 8, THREADS = 64 + 32 * EW, A_BYTES = BM * f4::KSB, MAX_SPLITS = 8;
+constexpr int BM = 128, EW = 8, THREADS = 64 + 32 * EW, A_BYTES = BM * f4::KSB, MAX_SPLITS = 4;  // (four tokens a CTA at least)
 constexpr int tokens_at_once(int bn) { return bn >= 64 ? 16 : 8; }  // of an epilogue warp
 constexpr int FUSED_STAGES = 16;  // of tokens, which stay, where the kernel quantises them itself
 constexpr int ring_bytes(int format) { return A_BYTES + f4::sf_bytes(format); }                    // a stage of the weight
 constexpr int token_bytes(int format, int bn) { return bn * f4::KSB + f4::sf_bytes(format); }      // and one of tokens
 // DEEP: as many stages as fit, for grids of at most a CTA an SM; else room for two CTAs an SM where the tile is narrow
 constexpr int stages(int bn, bool deep) { return bn == 16 ? (deep ? 8 : 4) : bn == 32 ? (deep ? 8 : 3) : bn == 64 ? 6 : 4; }
-constexpr int q_bytes(int bn) { return bn * BM * 4; }  // partial sums of a tile
+constexpr int q_bytes(int bn) { return BM * 4 * (bn + 4 * MAX_SPLITS); }  // partial sums of a tile
 constexpr int smem_bytes(int format, int bn, bool deep, bool fused) {
     return stages(bn, deep) * ring_bytes(format) + (fused ? FUSED_STAGES : stages(bn, deep)) * token_bytes(format, bn) + q_bytes(bn) + f4::BAR_BYTES +
            bn * 4 + 1024;
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
     static_assert(DEEP || TMEM_COLS <= 256, "tensor memory for two");
     extern __shared__ unsigned char smem_unaligned[];
     unsigned char* sm = smem_unaligned + ((1024u - (smem_u32(smem_unaligned) & 1023u)) & 1023u);
-    // [A of all stages][B of all stages][scales of A][scales of B][partial sums: split, token, channel][barriers][row factors]
+    // [A of all stages][B of all stages][scales of A][scales of B][partial sums: split, channel, token][barriers][row factors]
     unsigned char* sm_b = sm + STAGES * A_BYTES;
     unsigned char* sm_s = sm_b + TOKEN_STAGES * BN * f4::KSB;
     unsigned char* sm_t = sm_s + STAGES * SF;
@@ -248,14 +248,7 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
     const int q = warp & 3, half = (warp - 2) >> 2, ch = q * 32 + lane, n = n0 + ch;
     const int rows = min(BN, p.M - m0);
     float gw = 1.0f, bias = 0.0f;
-    // (residual reads are clamped to tokens and channels that exist, so that they need no branch and stay in flight together)
-    const T* res = p.residual ? static_cast<const T*>(p.residual) + (size_t)m0 * p.N + min(n, p.N - 1) : nullptr;
-    T* out = static_cast<T*>(p.y) + (size_t)m0 * p.N + n;
-    const auto result = [&](float sum, int t, float r) {
-        float y = fmaf(sum, gw * s_xg[t], bias);
-        if (p.relu2) y = relu_squared(y);
-        out[(size_t)t * p.N] = from_f<T>(y + r);
-    };
+    const int per = BN / p.splits, lg_per = 31 - __clz(per), pitch = per + 4;  // tokens that a CTA finishes; four more: no two lanes' 16 bytes meet in a bank
 
     if (warp == 0) {
         if (elect_lane()) {
@@ -315,9 +308,11 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
         if (clustered) cluster_wait();
         if (ok) {
             tc_fence_after();
-            const int per = BN / p.splits, lg_per = 31 - __clz(per);  // tokens that a CTA finishes
+            const T* res = p.residual ? static_cast<const T*>(p.residual) + (size_t)m0 * p.N + min(n, p.N - 1) : nullptr;
+            T* out = static_cast<T*>(p.y) + (size_t)m0 * p.N + n;
 #pragma unroll 1
             for (int c = TB * half; c < rows; c += 2 * TB) {
+                // (residual reads are clamped to tokens and channels that exist, so that they need no branch and stay in flight together)
                 T r[TB];
 #pragma unroll
                 for (int i = 0; i < TB; ++i) r[i] = from_f<T>(0.0f);
@@ -331,13 +326,19 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
                 tc_wait_ld();
                 if (!clustered) {
 #pragma unroll
-                    for (int i = 0; i < TB; ++i)
-                        if (c + i < rows && n < p.N) result(__uint_as_float(v[i]), c + i, to_f<T>(r[i]));
-                } else {
-#pragma unroll
                     for (int i = 0; i < TB; ++i) {
+                        float y = fmaf(__uint_as_float(v[i]), gw * s_xg[c + i], bias);
+                        if (p.relu2) y = relu_squared(y);
+                        if (c + i < rows && n < p.N) out[(size_t)(c + i) * p.N] = from_f<T>(y + to_f<T>(r[i]));
+                    }
+                } else {
+                    // four tokens at a time to the CTA that finishes them
+#pragma unroll
+                    for (int i = 0; i < TB; i += 4) {
                         const int to = (c + i) >> lg_per;
-                        if (c + i < rows) *cl.map_shared_rank(Q + ((split << lg_per) + (c + i) - (to << lg_per)) * BM + ch, to) = __uint_as_float(v[i]);
+                        if (c + i < rows)
+                            *reinterpret_cast<uint4*>(cl.map_shared_rank(Q, to) + (split * BM + ch) * pitch + (c + i) - (to << lg_per)) =
+                                make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                     }
                 }
             }
@@ -347,34 +348,43 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
     __syncwarp();
     if (clustered) {
         if (warp < 2) cluster_wait();
-        // the partial sums in the order of K, four tokens at a time, the first ones' residual requested under the barrier
-        const int per = BN / p.splits, t0 = split * per, t1 = min(rows, t0 + per);
-        const int tb = warp >= 2 && n < p.N ? t0 + half : t1;  // (the producer and MMA warps, and channels beyond N, have no token)
-        T r[4];
-        const auto residuals = [&](int t) {
+        // four tokens of this thread's channel a turn (one body: code that runs once waits for its instructions): the partial sums in the order of K, the
+        // residual two turns ahead
+        const int t0 = split << lg_per, count = min(rows - t0, per);
+        const T* res = p.residual ? static_cast<const T*>(p.residual) + (size_t)(m0 + t0) * p.N + min(n, p.N - 1) : nullptr;
+        T r[3][4];
+        const auto request = [&](T (&to)[4], int t) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = from_f<T>(0.0f);
-            if (res && t < t1) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = res[(size_t)min(t + 2 * i, t1 - 1) * p.N];
+            for (int i = 0; i < 4; ++i) {
+                to[i] = from_f<T>(0.0f);
+                if (res && t < count) to[i] = res[(size_t)min(t + i, count - 1) * p.N];  // (clamped to what exists: all four stay in flight)
             }
         };
-        residuals(tb);
+        if (warp >= 2) request(r[0], 4 * half), request(r[1], 4 * half + 8);
         cl.sync();
-        if (*abort_flag == 0)
-            for (int t = tb; t < t1; t += 8) {
-                if (t > tb) residuals(t);
-                float sum[4];
+        if (warp >= 2 && n < p.N && *abort_flag == 0) {  // (the producer and MMA warps, and channels beyond N, have no token)
+#pragma unroll 1
+            for (int t = 4 * half; t < count; t += 8) {
+                request(r[2], t + 16);
+                const float* src = Q + ch * pitch + t;
+                float4 sum = *reinterpret_cast<const float4*>(src);
+                for (int z = 1; z < p.splits; ++z) {
+                    const float4 more = *reinterpret_cast<const float4*>(src + z * BM * pitch);
+                    sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
+                }
+                const float4 gx = *reinterpret_cast<const float4*>(s_xg + t0 + t);
+                const float a[4] = {sum.x, sum.y, sum.z, sum.w}, g[4] = {gx.x, gx.y, gx.z, gx.w};
+                T* out = static_cast<T*>(p.y) + (size_t)(m0 + t0 + t) * p.N + n;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float* src = Q + (t + 2 * i < t1 ? t + 2 * i - t0 : 0) * BM + ch;
-                    sum[i] = src[0];
-                    for (int z = 1; z < p.splits; ++z) sum[i] += src[z * per * BM];
+                    float y = fmaf(a[i], gw * g[i], bias);
+                    if (p.relu2) y = relu_squared(y);
+                    if (t + i < count) *out = from_f<T>(y + to_f<T>(r[0][i]));
+                    out += p.N;
+                    r[0][i] = r[1][i], r[1][i] = r[2][i];
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (t + 2 * i < t1) result(sum[i], t + 2 * i, to_f<T>(r[i]));
             }
+        }
     }
     __syncthreads();
     if (warp == 1) {
