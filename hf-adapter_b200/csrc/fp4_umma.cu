@@ -185,8 +185,8 @@ __device__ __forceinline__ void quantise_tokens(const T* x, int64_t ldx, int M, 
 // FUSED: there is no quantiser, the tokens are quantised here under the first loads of the weight (quantise_tokens); everything waits for the
 // kernel before.
 // Bound by the weight's way from memory where there is much of it, else by the launch, the quantiser and the chain load, MMA, exchange, store.  us a
-// call, weights out of memory, nvfp4: 1 x 4096 -> 65536 (151 MB) 27.6 = 5.5 TB/s, 1 x 4096 -> 16384 (37.7 MB) 9.6, 1 x 4096 -> 4096
-// 6.6, 64 x 4096 -> 4096 8.6.
+// call, weights out of memory, nvfp4: 1 x 4096 -> 65536 (151 MB) 27.6 = 5.5 TB/s, 1 x 4096 -> 16384 (37.7 MB) 9.8, 1 x 4096 -> 4096
+// 5.7, 64 x 4096 -> 4096 8.3, 64 x 4096 -> 16384 12.6, 64 x 16384 -> 4096 14.7.
 template <int FORMAT, typename T, int BN, bool DEEP, bool FUSED>
 __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(const __grid_constant__ Fp4Maps maps, const Fp4Args p) {
     using namespace fs;
