@@ -332,7 +332,8 @@ __global__ void __launch_bounds__(fs::THREADS, DEEP ? 1 : 2) fp4_stream_kernel(c
                         if (c + i < rows && n < p.N) out[(size_t)(c + i) * p.N] = from_f<T>(y + to_f<T>(r[i]));
                     }
                 } else {
-                    // four tokens at a time to the CTA that finishes them
+                    // four tokens at a time to the CTA that finishes them (64 tokens, four CTAs: 24 KB leave a CTA at 14 bytes a cycle, which is what bounds
+                    // this; single words took a quarter longer)
 #pragma unroll
                     for (int i = 0; i < TB; i += 4) {
                         const int to = (c + i) >> lg_per;
