@@ -78,6 +78,7 @@ struct Shared {
         } w;
     };
 };
+static_assert(offsetof(Shared, owned) % 8 == 0, "its bins are read in pairs");
 constexpr int PICK_SHARED = (offsetof(Shared, count) + 15) / 16 * 16, FILTER_SHARED = (sizeof(Shared) + 15) / 16 * 16;
 }  // namespace lg
 
